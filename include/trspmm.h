@@ -39,6 +39,11 @@ extern "C" {
 
 typedef uint16_t trs_half; /* IEEE binary16 bits */
 
+/* Element types of the entries that take more than one (the first two as TRS_OUT_*). */
+#define TRS_TYPE_F32 0
+#define TRS_TYPE_F16 1
+#define TRS_TYPE_BF16 2
+
 /* The arrays block_sptc_2to4_online returns (block_online.cpp:844-870) that the forward pass
  * consumes (mGCN_online.cpp:760-800), with the value arrays already cast to fp16 as
  * mdataset2_online.py:151-153 does.  All pointers live in the same memory space. */
@@ -360,6 +365,29 @@ int trs_sddmm_plan_info(const trs_sddmm_plan* plan, long long* n_pairs, long lon
  * and whether it goes by cost. */
 int trs_sddmm_plan_shares(const trs_sddmm_plan* plan, int K, int* warps, unsigned* by_number, unsigned* by_cost, int* table);
 int trs_sddmm_plan_destroy(trs_sddmm_plan* plan);
+
+/* ---- embedding lookup and its gradient (no counterpart in the reference) ----------------------
+ * Learned feature rows, looked up by node or token ids:
+ *   out[i, :] = scale * table[id_i, :]            computed in fp32, rounded once to out_type
+ * table: [rows, F], out: [n, F], of TRS_TYPE_* each, rows `*_stride` >= F elements apart.  ids: [n] of 32 or
+ * (ids64 != 0) 64 bits.  An id equal to padding_id gives a row of zeros (TRS_NO_PADDING: no such id); an id outside
+ * [0, rows) gives a row of NaN, and nothing outside the table is read.  n = 0 does nothing.  `out` may not
+ * overlap the table.  Asynchronous on `stream`; allocates nothing.  Up to 2^31 - 65536 ids, 2^31 - 2 rows, 2^20 features
+ * (TRS_E_LIMIT beyond). */
+#define TRS_NO_PADDING INT64_MIN
+int trs_embedding(const void* table, int table_type, long long rows, long long table_stride, const void* ids, int ids64,
+                  long long n, int F, float scale, long long padding_id, void* out, int out_type, long long out_stride,
+                  void* stream);
+/* The gradient of the table: out[v, :] = scale * sum of grad[i, :] over the i with id_i = v, every row written (zeros
+ * where no id names it); with `accumulate` the sum is added to what the row holds (in fp32, rounded once), and rows that no
+ * id names are left as they are.  Ids equal to padding_id and ids outside [0, rows) contribute nothing.  The positions are
+ * sorted by id and summed in fp32 in an order that depends on the ids alone: no atomics, the same bits every time.
+ * `workspace`: trs_embedding_grad_workspace_bytes of 16-byte aligned device memory that no overlapping call uses;
+ * its contents need not be kept or cleared. */
+int trs_embedding_grad_workspace_bytes(long long n, long long rows, int F, size_t* bytes);
+int trs_embedding_grad(const void* grad, int grad_type, long long grad_stride, const void* ids, int ids64, long long n,
+                       long long rows, int F, float scale, long long padding_id, void* out, int out_type,
+                       long long out_stride, int accumulate, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -144,6 +144,12 @@ def load():
     lib.trs_build_array.restype = vp
     lib.trs_build_copy.argtypes = [vp, i32, vp, i32, vp]
     lib.trs_build_format.argtypes = [vp, C.POINTER(TrsFormat), vp]
+    i64, f32 = C.c_longlong, C.c_float
+    lib.trs_embedding.argtypes = [vp, i32, i64, i64, vp, i32, i64, i32, f32, i64, vp, i32, i64, vp]
+    lib.trs_embedding_grad_workspace_bytes.argtypes = [i64, i64, i32, C.POINTER(sz)]
+    lib.trs_embedding_grad.argtypes = [vp, i32, i64, vp, i32, i64, i64, i32, f32, i64, vp, i32, i64, i32, vp, sz, vp]
+    for name in ("trs_embedding", "trs_embedding_grad_workspace_bytes", "trs_embedding_grad"):
+        getattr(lib, name).restype = i32
     lib.trs_debug_stdsort_order.argtypes = [vp, i32, vp, C.POINTER(i32)]
     for name in ("trs_spmm_plan_create", "trs_spmm_plan_destroy", "trs_spmm_workspace_bytes", "trs_spmm_run",
                  "trs_spmm_launches", "trs_spmm_forward_host", "trs_resident_create", "trs_resident_forward",
