@@ -389,6 +389,33 @@ int trs_embedding_grad(const void* grad, int grad_type, long long grad_stride, c
                        long long rows, int F, float scale, long long padding_id, void* out, int out_type,
                        long long out_stride, int accumulate, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- log probabilities of given classes, entropy, alternatives (no counterpart in the reference) ---
+ * What the scores of a row over `classes` classes (node classes, or all nodes where links are predicted) say: with
+ * z = scale * x over the classes that may be chosen (mask != 0, score above -inf) and p = softmax(z),
+ *   logprobs[r] = log p[targets[r]],   entropy[r] = -sum p log p,
+ *   top_ids / top_logprobs[r, 0..top): the classes of the largest scores in descending order (the lowest class first among
+ *   equal scores) and their log probabilities,   stats[r] = {max x, sum exp(scale (x - max x))} for the gradient.
+ * x: [n, classes] of TRS_TYPE_*, rows `stride` >= classes elements apart, on any element boundary.  mask (may be NULL): one byte per class, rows
+ * mask_stride bytes apart (0: one row for all).  What stands in a masked place does not matter (NaN, infinities).  targets: [n] of 32 or (targets64 != 0) 64 bits; a
+ * target equal to ignore_id gives 0 (TRS_NO_IGNORE: no such id), one outside [0, classes) NaN, one that is masked -inf.  A row
+ * in which no class is left gives -inf, entropy 0 and alternatives -1 with -inf (as do alternatives beyond the number of
+ * classes left); a row in which a NaN or +inf is left gives NaN and alternatives -1.  Each output may be NULL
+ * (top_ids and top_logprobs only when top = 0, stats: 8-byte aligned).  scale > 0 and finite, top <= 32, classes <= 2^30,
+ * n < 2^31.  fp32 arithmetic whatever the type.  Asynchronous on `stream`; no workspace, allocates nothing. */
+#define TRS_NO_IGNORE INT64_MIN
+int trs_logprobs(const void* x, int type, long long n, int classes, long long stride, const void* targets, int targets64,
+                 long long ignore_id, const unsigned char* mask, long long mask_stride, float scale, int top,
+                 float* logprobs, float* entropy, float* top_logprobs, int32_t* top_ids, float* stats, void* stream);
+/* Gradient of the scores: from g_* = gradients of logprobs [n], entropy [n] and top_logprobs [n, top] (each may be NULL: 0),
+ * and the forward call's inputs and outputs (entropy is read where g_entropy is given, top_ids where g_top_logprobs is):
+ *   dx[r, j] = scale ( sum of g_c over the target and alternatives c = j  -  p_j (sum of all g_c + g_entropy (log p_j + entropy)) )
+ * of x's type, 0 where masked, for rows in which no class is left and for rows whose weights are all 0; NaN where the forward call gave NaN.
+ * Ignored targets and those outside [0, classes) have no weight.  dx may not overlap x. */
+int trs_logprobs_grad(const void* x, int type, long long n, int classes, long long stride, const void* targets, int targets64,
+                      long long ignore_id, const unsigned char* mask, long long mask_stride, float scale, int top,
+                      const int32_t* top_ids, const float* stats, const float* entropy, const float* g_logprobs,
+                      const float* g_entropy, const float* g_top_logprobs, void* dx, long long dx_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

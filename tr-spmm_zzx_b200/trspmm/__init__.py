@@ -15,4 +15,5 @@ from . import shard  # noqa: F401
 from .dataset import GCN_dataset_tcu_sptc_cuda_online, edges_to_csr, kernel_tcu_sptc_cuda_online  # noqa: F401
 from .autograd import DifferentiableSpmm, transpose_csr  # noqa: F401
 from .embedding import embedding, embedding_grad  # noqa: F401
+from .logprobs import ClassLogprobs, class_logprobs, class_logprobs_grad  # noqa: F401
 from . import reorder  # noqa: F401

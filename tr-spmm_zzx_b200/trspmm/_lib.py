@@ -148,7 +148,9 @@ def load():
     lib.trs_embedding.argtypes = [vp, i32, i64, i64, vp, i32, i64, i32, f32, i64, vp, i32, i64, vp]
     lib.trs_embedding_grad_workspace_bytes.argtypes = [i64, i64, i32, C.POINTER(sz)]
     lib.trs_embedding_grad.argtypes = [vp, i32, i64, vp, i32, i64, i64, i32, f32, i64, vp, i32, i64, i32, vp, sz, vp]
-    for name in ("trs_embedding", "trs_embedding_grad_workspace_bytes", "trs_embedding_grad"):
+    lib.trs_logprobs.argtypes = [vp, i32, i64, i32, i64, vp, i32, i64, vp, i64, f32, i32, vp, vp, vp, vp, vp, vp]
+    lib.trs_logprobs_grad.argtypes = [vp, i32, i64, i32, i64, vp, i32, i64, vp, i64, f32, i32, vp, vp, vp, vp, vp, vp, vp, i64, vp]
+    for name in ("trs_embedding", "trs_embedding_grad_workspace_bytes", "trs_embedding_grad", "trs_logprobs", "trs_logprobs_grad"):
         getattr(lib, name).restype = i32
     lib.trs_debug_stdsort_order.argtypes = [vp, i32, vp, C.POINTER(i32)]
     for name in ("trs_spmm_plan_create", "trs_spmm_plan_destroy", "trs_spmm_workspace_bytes", "trs_spmm_run",
