@@ -66,6 +66,12 @@ __device__ __forceinline__ Sums merge(Sums a, Sums b, float c) {
     return {m, a.S + b.S, a.T + b.T};
 }
 
+// The memory that a matrix of scores or a mask takes: an aligned piece inside may be read whole, whatever row its ends belong to.
+struct Extent {
+    uintptr_t begin, end;
+    __device__ __forceinline__ bool holds(const void* p, int bytes) const { return (uintptr_t)p >= begin && (uintptr_t)p + bytes <= end; }
+};
+
 // A row in pieces of 16 bytes on 16-byte boundaries; `head` elements of the first piece lie before the row.
 template <class T>
 struct Row {
@@ -73,28 +79,51 @@ struct Row {
     const T* x;
     const unsigned char* mask;   // null: none
     int head, pieces, classes;
-    __device__ __forceinline__ Row(const T* x_, const unsigned char* mask_, int classes_) : x(x_), mask(mask_), classes(classes_) {
-        head = (int)((uintptr_t)x_ % 16 / sizeof(T));
-        pieces = (head + classes_ + VEC - 1) / VEC;
+    Extent x_in, mask_in;
+    template <class Args>
+    __device__ __forceinline__ Row(const Args& a, long long r) : classes(a.classes), x_in(a.x_in), mask_in(a.mask_in) {
+        x = (const T*)a.x + r * a.stride;
+        mask = a.mask ? a.mask + r * a.mask_stride : nullptr;
+        head = (int)((uintptr_t)x % 16 / sizeof(T));
+        pieces = (head + classes + VEC - 1) / VEC;
     }
     __device__ __forceinline__ int first(int piece) const { return piece * VEC - head; }
     __device__ __forceinline__ bool inside(int j) const { return j >= 0 && j + VEC <= classes; }
     // scores as floats, -inf where there is none or it is masked
     __device__ __forceinline__ void load(int piece, float (&v)[VEC]) const {
         const int j = first(piece);
-        if (inside(j)) {
+        if (x_in.holds(x + j, 16)) {
             const Piece<T, VEC> p = *(const Piece<T, VEC>*)(x + j);
 #pragma unroll
             for (int k = 0; k < VEC; ++k) v[k] = as_float(p.v[k]);
-            if (mask) {
+        } else {   // the first piece of the matrix and its last
 #pragma unroll
-                for (int k = 0; k < VEC; ++k)
-                    if (!mask[j + k]) v[k] = -INFINITY;
+            for (int k = 0; k < VEC; ++k) v[k] = (unsigned)(j + k) < (unsigned)classes ? as_float(x[j + k]) : -INFINITY;
+        }
+        if (!inside(j)) {
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) v[k] = (unsigned)(j + k) < (unsigned)classes ? v[k] : -INFINITY;
+        }
+        if (mask) apply_mask(j, v);
+    }
+    __device__ __forceinline__ void apply_mask(int j, float (&v)[VEC]) const {
+        const unsigned char* at = mask + j;
+        const unsigned* word = (const unsigned*)((uintptr_t)at & ~(uintptr_t)3);
+        const unsigned shift = ((uintptr_t)at & 3) * 8;
+        constexpr int WORDS = VEC / 4 + 1;
+        if (mask_in.holds(word, 4 * WORDS)) {   // the bytes out of the aligned words around them
+            unsigned w[WORDS];
+#pragma unroll
+            for (int k = 0; k < WORDS; ++k) w[k] = __ldg(word + k);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                const unsigned four = __funnelshift_r(w[k / 4], w[k / 4 + 1], shift);
+                if (!(four >> (k % 4 * 8) & 0xff)) v[k] = -INFINITY;
             }
         } else {
 #pragma unroll
             for (int k = 0; k < VEC; ++k)
-                v[k] = j + k >= 0 && j + k < classes && (!mask || mask[j + k]) ? as_float(x[j + k]) : -INFINITY;
+                if ((unsigned)(j + k) < (unsigned)classes && !at[k]) v[k] = -INFINITY;
         }
     }
 };
@@ -108,6 +137,7 @@ struct Forward {
     long long ignore;
     const unsigned char* mask;
     long long mask_stride;
+    Extent x_in, mask_in;
     float scale, c;   // c = scale log2(e)
     int top;
     float *logprobs, *entropy, *top_logprobs;
@@ -174,7 +204,7 @@ template <class T, int THREADS>
 __global__ void __launch_bounds__(THREADS) k_row(const Forward a) {
     constexpr int WARPS = THREADS / 32, VEC = Row<T>::VEC;
     const long long r = blockIdx.x;
-    const Row<T> row((const T*)a.x + r * a.stride, a.mask ? a.mask + r * a.mask_stride : nullptr, a.classes);
+    const Row<T> row(a, r);
     Sums s{-INFINITY, 0.f, 0.f};
     int at = 0;   // where m is first
     for (int piece = threadIdx.x; piece < row.pieces; piece += THREADS) {
@@ -268,6 +298,85 @@ __global__ void __launch_bounds__(THREADS) k_row(const Forward a) {
 }
 
 // ----------------------------------------------------------------------------------------------
+// Short rows: a group of G lanes a row
+// ----------------------------------------------------------------------------------------------
+// The whole row is held in registers, PER pieces a lane (16 scores, or 32 for the longest), so the maximum comes first and the sums
+// after it.  An alternative is the group's maximum, then the lowest class that has it, taken out for the next one.
+constexpr int kShortThreads = 256;
+
+template <int G>
+__device__ __forceinline__ Sums group_sum(Sums s) {   // m is common
+#pragma unroll
+    for (int o = G / 2; o; o /= 2) {
+        s.S += __shfl_xor_sync(0xffffffffu, s.S, o);
+        s.T += __shfl_xor_sync(0xffffffffu, s.T, o);
+    }
+    return s;
+}
+
+template <class T, int G, int PER>
+__global__ void __launch_bounds__(kShortThreads) k_short_rows(const Forward a) {
+    constexpr int VEC = Row<T>::VEC;
+    const int g = threadIdx.x % G;
+    const long long r0 = ((long long)blockIdx.x * kShortThreads + threadIdx.x) / G, r = r0 < a.n ? r0 : a.n - 1;   // lanes stay together
+    const Row<T> row(a, r);
+    float v[PER][VEC];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        if (g + i * G < row.pieces) {
+            row.load(g + i * G, v[i]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) v[i][k] = -INFINITY;
+        }
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) m = max_nan(m, v[i][k]);
+#pragma unroll
+    for (int o = G / 2; o; o /= 2) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    Sums s{m, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+            const float d = fmaxf((v[i][k] - m) * a.c, kFar), e = exp_2(d);
+            s.S += e;
+            s.T = fmaf(e, d, s.T);
+        }
+    s = group_sum<G>(s);
+    if (g == 0 && r == r0) write_row<T>(a, r, row.x, row.mask, s);
+    const bool broken = !(m < INFINITY);
+    for (int k = 0; k < a.top; ++k) {
+        if (k) {
+            m = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) m = fmaxf(m, v[i][q]);
+#pragma unroll
+            for (int o = G / 2; o; o /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        }
+        int at = 0x7fffffff;
+#pragma unroll
+        for (int i = PER; i-- > 0;)
+#pragma unroll
+            for (int q = VEC; q-- > 0;)
+                if (v[i][q] == m) at = row.first(g + i * G) + q;
+#pragma unroll
+        for (int o = G / 2; o; o /= 2) at = min(at, __shfl_xor_sync(0xffffffffu, at, o));
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+#pragma unroll
+            for (int q = 0; q < VEC; ++q)
+                if (row.first(g + i * G) + q == at) v[i][q] = -INFINITY;
+        if (k % G == g && r == r0) write_top(a, r, k, broken || m == -INFINITY ? 0 : key_of(m, at), s);
+    }
+}
+
+// ----------------------------------------------------------------------------------------------
 // Gradient
 // ----------------------------------------------------------------------------------------------
 struct Backward {
@@ -279,6 +388,7 @@ struct Backward {
     long long ignore;
     const unsigned char* mask;
     long long mask_stride;
+    Extent x_in, mask_in;
     float scale, c;
     int top;
     const int* top_ids;
@@ -365,7 +475,7 @@ template <class T>
 __global__ void __launch_bounds__(kGradThreads) k_row_grad(const Backward a, int parts) {
     const long long r = blockIdx.x / parts;
     const int part = (int)(blockIdx.x - r * parts);
-    const Row<T> row((const T*)a.x + r * a.stride, a.mask ? a.mask + r * a.mask_stride : nullptr, a.classes);
+    const Row<T> row(a, r);
     T* dx = (T*)a.dx + r * a.dx_stride;
     const RowGrad g = row_grad(a, r);
     const int p0 = part * kGradThreads * kGradPieces, p1 = min(row.pieces, p0 + kGradThreads * kGradPieces);
@@ -378,6 +488,49 @@ __global__ void __launch_bounds__(kGradThreads) k_row_grad(const Backward a, int
         const int piece = (int)((j + row.head) / Row<T>::VEC);
         if (piece >= p0 && piece < p1) write_own<T>(a, r, g, row, dx, j);
     }
+}
+
+template <class T, int G, int PER>
+__global__ void __launch_bounds__(kShortThreads) k_short_rows_grad(const Backward a) {
+    const int g = threadIdx.x % G;
+    const long long r = ((long long)blockIdx.x * kShortThreads + threadIdx.x) / G;
+    const bool in = r < a.n;
+    const Row<T> row(a, in ? r : 0);
+    T* dx = (T*)a.dx + (in ? r : 0) * a.dx_stride;
+    const RowGrad w = row_grad(a, in ? r : 0);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+        if (in && g + i * G < row.pieces) write_piece<T>(a, w, row, dx, g + i * G);
+    __syncwarp();   // behind the lanes of the row, as in k_row_grad
+    if (!in || w.zero) return;
+    for (int k = g; k < 1 + (a.g_top ? a.top : 0); k += G) {
+        const long long j = k ? a.top_ids[r * a.top + k - 1] : a.g_logprobs ? load_target(a.target, a.target64, r) : -1;
+        if (j < 0 || j >= a.classes || (k == 0 && !target_counts(a, j))) continue;
+        write_own<T>(a, r, w, row, dx, j);
+    }
+}
+
+// Lanes and pieces per lane that hold a row of so many pieces; beyond 32 x 2 x (16 scores) a row is a CTA's.
+constexpr int kShortScores = 16;
+template <class T, class Fn>
+int with_short(int pieces, Fn fn) {
+    constexpr int PER = kShortScores / Row<T>::VEC;
+    if (pieces <= PER) return fn(std::integral_constant<int, 1>(), std::integral_constant<int, PER>());
+    if (pieces <= 2 * PER) return fn(std::integral_constant<int, 2>(), std::integral_constant<int, PER>());
+    if (pieces <= 4 * PER) return fn(std::integral_constant<int, 4>(), std::integral_constant<int, PER>());
+    if (pieces <= 8 * PER) return fn(std::integral_constant<int, 8>(), std::integral_constant<int, PER>());
+    if (pieces <= 16 * PER) return fn(std::integral_constant<int, 16>(), std::integral_constant<int, PER>());
+    if (pieces <= 32 * PER) return fn(std::integral_constant<int, 32>(), std::integral_constant<int, PER>());
+    return fn(std::integral_constant<int, 32>(), std::integral_constant<int, 2 * PER>());
+}
+template <class T>
+constexpr int kShortPieces = 64 * kShortScores / Row<T>::VEC;
+// Pieces of a row, wherever it begins.
+template <class T>
+int most_pieces(int classes) { return (int)ceil_div64((long long)classes + Row<T>::VEC - 1, Row<T>::VEC); }
+
+Extent extent(const void* p, long long rows, long long stride, long long width, int size) {
+    return {(uintptr_t)p, (uintptr_t)p + (size_t)((rows - 1) * stride + width) * size};
 }
 
 int check(const void* x, int type, long long n, int classes, long long stride, const void* mask, long long mask_stride, float scale,
@@ -401,11 +554,17 @@ extern "C" int trs_logprobs(const void* x, int type, long long n, int classes, l
     if (rc) return rc;
     if (n == 0) return TRS_OK;
     if ((logprobs && !targets) || (top && (!top_logprobs || !top_ids)) || (uintptr_t)stats % 8) return TRS_E_ARG;
-    const Forward a{x, n, stride, classes, targets, targets64, ignore_id, mask, mask_stride, scale, scale * kLog2e, top, logprobs, entropy,
+    const Forward a{x, n, stride, classes, targets, targets64, ignore_id, mask, mask_stride, extent(x, n, stride, classes, type_bytes(type)), extent(mask, n, mask_stride, classes, 1), scale, scale * kLog2e, top, logprobs, entropy,
                     top_logprobs, top_ids, (float2*)stats};
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        const int pieces = ceil_div(classes, Row<T>::VEC);
+        const int pieces = most_pieces<T>(classes);
+        if (pieces <= kShortPieces<T>)
+            return with_short<T>(pieces, [&](auto g, auto per) {
+                constexpr int G = decltype(g)::value;
+                return launch(k_short_rows<T, G, decltype(per)::value>, dim3((unsigned)ceil_div64(n * G, kShortThreads)), kShortThreads, 0,
+                              (cudaStream_t)stream, a);
+            });
         if (pieces <= 256) return launch(k_row<T, 128>, dim3((unsigned)n), 128, 0, (cudaStream_t)stream, a);
         return launch(k_row<T, 512>, dim3((unsigned)n), 512, 0, (cudaStream_t)stream, a);
     });
@@ -422,10 +581,17 @@ extern "C" int trs_logprobs_grad(const void* x, int type, long long n, int class
     if (n == 0) return TRS_OK;
     if (!dx || (uintptr_t)dx % type_bytes(type) || !stats || (uintptr_t)stats % 8) return TRS_E_ARG;
     if ((g_logprobs && !targets) || (g_entropy && !entropy) || (g_top_logprobs && (!top_ids || !top))) return TRS_E_ARG;
-    const Backward a{x, n, stride, classes, targets, targets64, ignore_id, mask, mask_stride, scale, scale * kLog2e, top, top_ids,
+    const Backward a{x, n, stride, classes, targets, targets64, ignore_id, mask, mask_stride, extent(x, n, stride, classes, type_bytes(type)), extent(mask, n, mask_stride, classes, 1), scale, scale * kLog2e, top, top_ids,
                      (const float2*)stats, entropy, g_logprobs, g_entropy, g_top_logprobs, dx, dx_stride};
     return with_type(type, [&](auto t) {
         using T = decltype(t);
+        const int pieces = most_pieces<T>(classes);
+        if (pieces <= kShortPieces<T>)
+            return with_short<T>(pieces, [&](auto g, auto per) {
+                constexpr int G = decltype(g)::value;
+                return launch(k_short_rows_grad<T, G, decltype(per)::value>, dim3((unsigned)ceil_div64(n * G, kShortThreads)), kShortThreads,
+                              0, (cudaStream_t)stream, a);
+            });
         const long long parts = ceil_div64((long long)classes + Row<T>::VEC - 1, (long long)Row<T>::VEC * kGradThreads * kGradPieces);
         if (n * parts > 0x7fffffffll) return (int)TRS_E_LIMIT;
         return launch(k_row_grad<T>, dim3((unsigned)(n * parts)), kGradThreads, 0, (cudaStream_t)stream, a, (int)parts);
