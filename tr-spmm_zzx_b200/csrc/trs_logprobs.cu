@@ -35,11 +35,6 @@ __device__ __forceinline__ float key_score(Key k) {
 }
 __device__ __forceinline__ int key_class(Key k) { return (int)~(unsigned)k; }
 
-__device__ __forceinline__ float max_nan(float a, float b) {   // NaN where one is
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
 __device__ __forceinline__ float exp_2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -93,9 +88,7 @@ struct Row {
     __device__ __forceinline__ void load(int piece, float (&v)[VEC]) const {
         const int j = first(piece);
         if (x_in.holds(x + j, 16)) {
-            const Piece<T, VEC> p = *(const Piece<T, VEC>*)(x + j);
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) v[k] = as_float(p.v[k]);
+            as_floats(*(const Piece<T, VEC>*)(x + j), v);
         } else {   // the first piece of the matrix and its last
 #pragma unroll
             for (int k = 0; k < VEC; ++k) v[k] = (unsigned)(j + k) < (unsigned)classes ? as_float(x[j + k]) : -INFINITY;
@@ -192,109 +185,350 @@ __device__ __forceinline__ void warp_top(const Key* keys, int n, int top, Key* o
     __syncwarp();
 }
 
+// The same by all threads of a CTA or a warp (`me` of `threads`), each key to the place that its rank gives it; out is 0 before.  For short lists.
+__device__ __forceinline__ void rank_top(const Key* keys, int n, int top, Key* out, int me, int threads) {
+    for (int i = me; i < n; i += threads) {
+        const Key k = keys[i];
+        int rank = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) rank += keys[j] > k;
+        if (k != 0 && rank < top) out[rank] = k;
+    }
+}
+
+// The warp's keys in descending order over the lanes.
+__device__ __forceinline__ Key warp_sort(Key k) {
+    const int lane = threadIdx.x % 32;
+#pragma unroll
+    for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+        for (int o = size / 2; o; o /= 2) {
+            const Key other = __shfl_xor_sync(0xffffffffu, k, o);
+            const bool larger = ((lane & o) == 0) == ((lane & size) == 0);   // (lane & 32 is 0: the last merge descends)
+            if ((other > k) == larger) k = other;
+        }
+    return k;
+}
+
 // ----------------------------------------------------------------------------------------------
 // One CTA a row
 // ----------------------------------------------------------------------------------------------
-// The maximum of each thread's part and where it is first come with the sums for nothing.  The top-th largest of those maxima, K, bounds the
-// row's top-th score from below, and only the `top` threads with maxima from K on can hold scores from K on: their parts are
-// read again (from L2), and the few scores that reach K are sorted out by one warp.
-constexpr int kCandidates = 1024;
+// A thread takes TURN pieces, THREADS apart, at a time: their loads are under way together, their maximum is compared once with the
+// part's, and the sums go two scores an instruction.  The pieces that the row's ends cut come last.
+//
+// Alternatives: each thread's largest score and the piece it is first in come with the sums for nothing.  The key (score, last class of that
+// piece) is at most the key of a score of the row, so the top-th largest of the threads' keys - of 32 groups of threads, which
+// one sort of a warp gives - is at most the row's top-th largest: K.  Only threads whose key (score, first class of the piece)
+// reaches K can hold scores from K on, little more than `top` of them.  That piece is read again - all pieces of the thread where the
+// second largest of its pieces' maxima reaches K too - and the few scores that reach K are put in order by their ranks.
+//
+// Few rows are split over the CTAs of a cluster (`parts`), which hand their sums and alternatives to the first one.
+constexpr int kCandidates = 1024, kTurn = 4, kMaxParts = 8;
 
-template <class T, int THREADS>
-__global__ void __launch_bounds__(THREADS) k_row(const Forward a) {
-    constexpr int WARPS = THREADS / 32, VEC = Row<T>::VEC;
-    const long long r = blockIdx.x;
-    const Row<T> row(a, r);
-    Sums s{-INFINITY, 0.f, 0.f};
-    int at = 0;   // where m is first
-    for (int piece = threadIdx.x; piece < row.pieces; piece += THREADS) {
-        float v[VEC];
-        row.load(piece, v);
-        float m = s.m;
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) m = max_nan(m, v[k]);
-        if (!(m <= s.m)) {
-            rescale(s, m, a.c);
-#pragma unroll
-            for (int k = VEC; k-- > 0;)
-                if (v[k] == m) at = row.first(piece) + k;
-        }
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-            const float d = fmaxf((v[k] - m) * a.c, kFar), e = exp_2(d);
-            s.S += e;
-            s.T = fmaf(e, d, s.T);
-        }
+// A thread's sums with two accumulators, relative to `ref`: a maximum up to 2^kSlack below the present one (e^(d) stays far from
+// overflow, and sums are rescaled once or twice in a row instead of at every new maximum); and where the maximum is first.
+constexpr float kSlack = 16.f;
+struct Running {
+    float m = -INFINITY, ref = -INFINITY;
+    float second = -INFINITY;   // largest of the other pieces' maxima
+    float2 S = {0.f, 0.f}, T = {0.f, 0.f};
+    int at = 0x7fffffff;   // a piece
+    __device__ __forceinline__ Sums sums(float c) const {
+        Sums s{ref, S.x + S.y, T.x + T.y};
+        rescale(s, m, c);
+        return s;
     }
-    __shared__ Sums s_part[WARPS];
-    __shared__ Key s_key[THREADS], s_found[kCandidates], s_best[kMaxTop];
-    __shared__ int s_sel[kMaxTop], s_count[2];
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const Key mine = s.m > -INFINITY ? key_of(s.m, at) : 0;
-    Sums w = s;
-#pragma unroll
-    for (int o = 16; o; o /= 2) {
-        const Sums other{__shfl_xor_sync(0xffffffffu, w.m, o), __shfl_xor_sync(0xffffffffu, w.S, o), __shfl_xor_sync(0xffffffffu, w.T, o)};
-        w = merge(w, other, a.c);
+    // before scores up to `top` are added
+    __device__ __forceinline__ void make_room(float top, float c) {
+        if ((top - ref) * c <= kSlack) return;
+        Sums s{ref, S.x + S.y, T.x + T.y};
+        rescale(s, top, c);
+        ref = top;
+        S = make_float2(s.S, 0.f);
+        T = make_float2(s.T, 0.f);
     }
-    if (lane == 0) s_part[warp] = w;
-    if (a.top) s_key[threadIdx.x] = mine;
-    if (threadIdx.x < 2) s_count[threadIdx.x] = 0;
-    __syncthreads();
-    Sums all = s_part[0];
-    for (int k = 1; k < WARPS; ++k) all = merge(all, s_part[k], a.c);
-    if (threadIdx.x == 0) write_row<T>(a, r, row.x, row.mask, all);
-    if (!a.top) return;
-
-    if (warp == 0) warp_top(s_key, THREADS, a.top, s_best);
-    __syncthreads();
-    const Key bound = s_best[a.top - 1];
-    if (mine != 0 && mine >= bound) s_sel[atomicAdd(&s_count[0], 1)] = threadIdx.x;   // at most `top`: keys differ
-    __syncthreads();
-    const int turns = (row.pieces + THREADS - 1) / THREADS, items = s_count[0] * turns;
-    for (int i = threadIdx.x; i < items; i += THREADS) {
-        const int piece = s_sel[i / turns] + i % turns * THREADS;
-        if (piece >= row.pieces) continue;
-        float v[VEC];
-        row.load(piece, v);
+    // NEAR: no score is -inf, or so far below m that d is; otherwise T is NaN afterwards
+    template <bool NEAR, class E, int N>
+    __device__ __forceinline__ void add(const Piece<E, N>& x, float2 minus, float2 c2) {
+        float v[N];
+        as_floats(x, v);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-            if (!(v[k] > -INFINITY)) continue;
-            const Key key = key_of(v[k], row.first(piece) + k);
-            if (key < bound) continue;
-            const int to = atomicAdd(&s_count[1], 1);
-            if (to < kCandidates) s_found[to] = key;
-        }
-    }
-    __syncthreads();
-    if (s_count[1] <= kCandidates) {
-        if (warp == 0) warp_top(s_found, s_count[1], a.top, s_best);
-    } else {
-        // more scores than the list holds (rows in which a few threads' parts have nearly all of the largest ones): one round
-        // over the row for each alternative
-        Key last = ~0ull;
-        for (int k = 0; k < a.top; ++k) {
-            Key best = 0;
-            for (int piece = threadIdx.x; piece < row.pieces; piece += THREADS) {
-                float v[VEC];
-                row.load(piece, v);
-#pragma unroll
-                for (int q = 0; q < VEC; ++q) {
-                    const Key key = v[q] > -INFINITY ? key_of(v[q], row.first(piece) + q) : 0;
-                    if (key < last && key > best) best = key;
-                }
+        for (int k = 0; k < N; k += 2) {
+            float2 d = __fmul2_rn(__fadd2_rn(make_float2(v[k], v[k + 1]), minus), c2);
+            if (!NEAR) {
+                d.x = fmaxf(d.x, kFar);
+                d.y = fmaxf(d.y, kFar);
             }
-            best = warp_max(best);
-            __syncthreads();
-            if (lane == 0) s_key[warp] = best;
-            __syncthreads();
-            last = 0;
-            for (int q = 0; q < WARPS; ++q) last = s_key[q] > last ? s_key[q] : last;
-            if (threadIdx.x == 0) s_best[k] = last;
+            const float2 e = make_float2(exp_2(d.x), exp_2(d.y));
+            S = __fadd2_rn(S, e);
+            T = __ffma2_rn(e, d, T);
         }
     }
+};
+template <class T, int THREADS, bool MASKED>
+__global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_row(const Forward a, int parts) {
+    constexpr int WARPS = THREADS / 32, VEC = Row<T>::VEC, TURN = kTurn, WORDS = VEC / 4 + 1;
+    const long long r = blockIdx.x / parts;
+    const int part = (int)(blockIdx.x - r * parts);
+    const Row<T> row(a, r);
+    const int per = (row.pieces + parts - 1) / parts, p0 = min(row.pieces, part * per), p1 = min(row.pieces, p0 + per);
+    // pieces [q0, q1) lie inside the row
+    int q0 = max(p0, row.head ? 1 : 0);
+    int q1 = min(p1, (row.head + row.classes) / VEC);
+    const unsigned char* mask_word = nullptr;
+    unsigned mask_shift = 0;
+    if (MASKED) {
+        mask_word = (const unsigned char*)((uintptr_t)(row.mask - row.head) & ~(uintptr_t)3);
+        mask_shift = ((uintptr_t)(row.mask - row.head) & 3) * 8;
+    }
+    const bool mask_even = MASKED && (uintptr_t)(row.mask - row.head) % VEC == 0;   // a piece's bytes in one load
+    const int last_word = mask_shift ? VEC : VEC - 4;   // the last word with a byte of the piece
+    q0 = min(q0, p1);
+    q1 = max(q1, q0);
+    const float2 c2 = make_float2(a.c, a.c);
+    Running s;
+    struct Raw {
+        Piece<T, VEC> x;
+        unsigned bits[WORDS];
+    };
+    auto fetch_mask = [&](Raw& w, int piece) {
+        if (MASKED && mask_even) {
+            const Piece<unsigned, VEC / 4> b = *(const Piece<unsigned, VEC / 4>*)(mask_word + (size_t)piece * VEC);
+#pragma unroll
+            for (int k = 0; k < VEC / 4; ++k) w.bits[k] = b.v[k];
+            w.bits[VEC / 4] = 0;
+        } else if (MASKED) {
+#pragma unroll
+            for (int k = 0; k < WORDS; ++k)
+                w.bits[k] = __ldg((const unsigned*)(mask_word + (size_t)piece * VEC + (k < WORDS - 1 ? 4 * k : last_word)));
+        }
+    };
+    auto fetch = [&](int piece) {
+        Raw w;
+        w.x = *(const Piece<T, VEC>*)(row.x + row.first(piece));
+        fetch_mask(w, piece);
+        return w;
+    };
+    auto masked = [&](Raw& w) {
+        if (MASKED) {
+#pragma unroll
+            for (int k = 0; k < VEC / 4; ++k) mask_four(w.x, 4 * k, __funnelshift_r(w.bits[k], w.bits[k + 1], mask_shift));
+        }
+    };
+    // one turn; `near`: no difference is bounded, and the answer is whether none needed to be (otherwise nothing is added)
+    auto take = [&](auto near, int base) {
+        constexpr bool NEAR = decltype(near)::value;
+        Raw w[TURN];
+#pragma unroll
+        for (int u = 0; u < TURN; ++u) w[u] = fetch(base + u * THREADS);
+        float pm[TURN], m = s.m;
+#pragma unroll
+        for (int u = 0; u < TURN; ++u) {
+            masked(w[u]);
+            pm[u] = max_of(w[u].x);
+            m = max_nan(m, pm[u]);
+        }
+        if (a.top) {
+            float first = s.m;
+#pragma unroll
+            for (int u = 0; u < TURN; ++u) {
+                s.second = fmaxf(s.second, fminf(first, pm[u]));
+                first = fmaxf(first, pm[u]);
+            }
+            if (m > s.m) {
+#pragma unroll
+                for (int u = TURN; u-- > 0;)
+                    if (pm[u] == m) s.at = base + u * THREADS;
+            }
+        }
+        s.m = m;
+        s.make_room(m, a.c);
+        const float2 minus = make_float2(-s.ref, -s.ref), S0 = s.S, T0 = s.T;
+#pragma unroll
+        for (int u = 0; u < TURN; ++u) s.template add<NEAR>(w[u].x, minus, c2);
+        const float sum = s.T.x + s.T.y;
+        if (NEAR && !(sum == sum)) {
+            s.S = S0;
+            s.T = T0;
+            return false;
+        }
+        return true;
+    };
+    auto take_one = [&](int piece) {
+        Raw w = fetch(piece);
+        masked(w);
+        const float pm = max_of(w.x);
+        s.second = fmaxf(s.second, fminf(s.m, pm));
+        if (pm > s.m) s.at = piece;
+        s.m = max_nan(s.m, pm);
+        s.make_room(s.m, a.c);
+        s.template add<false>(w.x, make_float2(-s.ref, -s.ref), c2);
+    };
+    int base = q0 + threadIdx.x;
+    const int last = q1 - (TURN - 1) * THREADS;
+    bool near = !MASKED;
+    while (near && base < last) {
+        near = take(std::true_type(), base);
+        if (near) base += TURN * THREADS;
+    }
+    for (; base < last; base += TURN * THREADS) take(std::false_type(), base);
+    for (; base < q1; base += THREADS) take_one(base);
+    const int cut = q0 - p0 + p1 - q1;   // pieces that are not whole
+    auto cut_piece = [&](int i) { return i < q0 - p0 ? p0 + i : q1 + i - (q0 - p0); };
+    if (THREADS - 1 - (int)threadIdx.x < cut) {
+        float v[VEC];
+        const int piece = cut_piece(THREADS - 1 - threadIdx.x);
+        row.load(piece, v);
+        Piece<T, VEC> x;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) x.v[k] = from_float<T>(v[k]);   // what it was
+        const float pm = max_of(x);
+        s.second = fmaxf(s.second, fminf(s.m, pm));
+        if (pm > s.m || (pm == s.m && piece < s.at)) s.at = piece;
+        s.m = max_nan(s.m, pm);
+        s.make_room(s.m, a.c);
+        s.template add<false>(x, make_float2(-s.ref, -s.ref), c2);
+    }
+    __shared__ Sums s_part[WARPS], s_all;
+    __shared__ Key s_key[THREADS], s_found[kCandidates], s_best[kMaxTop];
+    __shared__ Key s_bound;
+    __shared__ int s_sel[THREADS], s_count[2];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    auto warp_sum = [&](Sums w, int lanes) {
+        for (int o = lanes / 2; o; o /= 2) {
+            const Sums other{__shfl_xor_sync(0xffffffffu, w.m, o), __shfl_xor_sync(0xffffffffu, w.S, o), __shfl_xor_sync(0xffffffffu, w.T, o)};
+            w = merge(w, other, a.c);
+        }
+        return w;
+    };
+    const Sums w = warp_sum(s.sums(a.c), 32);
+    if (lane == 0) s_part[warp] = w;
+    const bool some = s.m > -INFINITY;
+    if (a.top) s_key[threadIdx.x] = some ? key_of(s.m, row.first(s.at) + VEC - 1) : 0;
+    if (threadIdx.x < 2) s_count[threadIdx.x] = 0;
+    if (threadIdx.x < a.top) s_best[threadIdx.x] = 0;
     __syncthreads();
-    for (int k = threadIdx.x; k < a.top; k += THREADS) write_top(a, r, k, s_best[k], all);
+    if (warp == WARPS - 1) {
+        const Sums all = warp_sum(s_part[lane % WARPS], WARPS);
+        if (lane == 0) {
+            s_all = all;
+            if (parts == 1) write_row<T>(a, r, row.x, row.mask, all);
+        }
+    }
+    if (a.top) {
+        if (warp == 0) {
+            Key best = 0;
+#pragma unroll
+            for (int i = 0; i < WARPS; ++i) best = s_key[i * 32 + lane] > best ? s_key[i * 32 + lane] : best;
+            best = __shfl_sync(0xffffffffu, warp_sort(best), a.top - 1);
+            if (best == 0) {   // fewer groups have a score: the threads' own keys
+                warp_top(s_key, THREADS, a.top, s_found);
+                best = s_found[a.top - 1];
+            }
+            if (lane == 0) s_bound = best;
+        }
+        __syncthreads();
+        const Key bound = s_bound;
+        const float least = bound ? key_score(bound) : -INFINITY;
+        auto keep = [&](const float (&v)[VEC], int piece) {
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                if (!(v[k] > -INFINITY)) continue;
+                const Key key = key_of(v[k], row.first(piece) + k);
+                if (key < bound) continue;
+                const int to = atomicAdd(&s_count[1], 1);
+                if (to < kCandidates) s_found[to] = key;
+            }
+        };
+        if (some && key_of(s.m, max(row.first(s.at), 0)) >= bound) {
+            if (s.second >= least) {
+                s_sel[atomicAdd(&s_count[0], 1)] = threadIdx.x;
+            } else if (s.at >= q0 && s.at < q1) {   // no other piece of the thread's reaches K
+                Raw w = fetch(s.at);
+                masked(w);
+                float v[VEC];
+                as_floats(w.x, v);
+                keep(v, s.at);
+            }
+        }
+        __syncthreads();
+        const int turns = (q1 - q0 + THREADS - 1) / THREADS, items = s_count[0] * turns;
+        for (int i0 = threadIdx.x; i0 < items; i0 += kTurn * THREADS) {
+            Raw w[kTurn];
+            int at[kTurn];
+#pragma unroll
+            for (int u = 0; u < kTurn; ++u) {
+                const int i = i0 + u * THREADS, sel = i / turns;
+                at[u] = i < items ? q0 + s_sel[sel] + (i - sel * turns) * THREADS : q1;
+                if (at[u] < q1) w[u] = fetch(at[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < kTurn; ++u) {
+                if (at[u] >= q1) continue;
+                masked(w[u]);
+                if (max_of(w[u].x) < least) continue;
+                float v[VEC];
+                as_floats(w[u].x, v);
+                keep(v, at[u]);
+            }
+        }
+        if (THREADS - 1 - (int)threadIdx.x < cut) {   // the cut pieces too, whoever had them
+            float v[VEC];
+            const int piece = cut_piece(THREADS - 1 - threadIdx.x);
+            row.load(piece, v);
+            keep(v, piece);
+        }
+        __syncthreads();
+        if (s_count[1] <= 256) {
+            rank_top(s_found, s_count[1], a.top, s_best, threadIdx.x, THREADS);
+        } else if (s_count[1] <= kCandidates) {
+            if (warp == 0) warp_top(s_found, s_count[1], a.top, s_best);
+        } else {
+            // more scores than the list holds (rows in which a few threads' parts have nearly all of the largest ones): one round
+            // over the row for each alternative
+            Key last = ~0ull;
+            for (int k = 0; k < a.top; ++k) {
+                Key best = 0;
+                for (int piece = p0 + threadIdx.x; piece < p1; piece += THREADS) {
+                    float v[VEC];
+                    row.load(piece, v);
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) {
+                        const Key key = v[q] > -INFINITY ? key_of(v[q], row.first(piece) + q) : 0;
+                        if (key < last && key > best) best = key;
+                    }
+                }
+                best = warp_max(best);
+                __syncthreads();
+                if (lane == 0) s_key[warp] = best;
+                __syncthreads();
+                last = 0;
+                for (int q = 0; q < WARPS; ++q) last = s_key[q] > last ? s_key[q] : last;
+                if (threadIdx.x == 0) s_best[k] = last;
+            }
+        }
+    }
+    if (parts > 1) {
+        const auto cluster = cooperative_groups::this_cluster();
+        cluster.sync();
+        if (part == 0 && warp == 0) {
+            const Sums all = warp_sum(*cluster.map_shared_rank(&s_all, lane % parts), parts);
+            for (int i = lane; i < parts * a.top; i += 32) s_found[i] = cluster.map_shared_rank(s_best, i / a.top)[i % a.top];
+            __syncwarp();
+            if (lane < a.top) s_best[lane] = 0;
+            __syncwarp();
+            if (a.top) rank_top(s_found, parts * a.top, a.top, s_best, lane, 32);
+            if (lane == 0) {
+                s_all = all;
+                write_row<T>(a, r, row.x, row.mask, all);
+            }
+        }
+        cluster.sync();   // nobody leaves while its shared memory is read
+        if (part) return;
+    } else if (a.top) {
+        __syncthreads();
+    }
+    for (int k = threadIdx.x; k < a.top; k += THREADS) write_top(a, r, k, s_best[k], s_all);
 }
 
 // ----------------------------------------------------------------------------------------------
@@ -469,23 +703,65 @@ __device__ __forceinline__ void write_piece(const Backward& a, const RowGrad& g,
     }
 }
 
-constexpr int kGradThreads = 256, kGradPieces = 8;   // pieces per thread
+constexpr int kGradThreads = 256, kGradTurn = 4, kGradPieces = 2 * kGradTurn;   // pieces per thread: turns of four whose loads are under way together
 
-template <class T>
+template <class T, bool MASKED>
 __global__ void __launch_bounds__(kGradThreads) k_row_grad(const Backward a, int parts) {
+    constexpr int VEC = Row<T>::VEC;
     const long long r = blockIdx.x / parts;
     const int part = (int)(blockIdx.x - r * parts);
     const Row<T> row(a, r);
     T* dx = (T*)a.dx + r * a.dx_stride;
     const RowGrad g = row_grad(a, r);
-    const int p0 = part * kGradThreads * kGradPieces, p1 = min(row.pieces, p0 + kGradThreads * kGradPieces);
-    for (int piece = p0 + threadIdx.x; piece < p1; piece += kGradThreads) write_piece<T>(a, g, row, dx, piece);
-    if (g.zero) return;
+    const int per = (row.pieces + parts - 1) / parts, p0 = min(row.pieces, part * per), p1 = min(row.pieces, p0 + per);
+    // whole pieces whose places in dx are aligned as in x
+    const bool straight = (uintptr_t)(dx - row.head) % 16 == 0;
+    const int q0 = straight && !MASKED ? max(p0, row.head ? 1 : 0) : p1, q1 = min(p1, (row.head + row.classes) / VEC);
+    if (g.zero) {
+        for (int piece = p0 + threadIdx.x; piece < p1; piece += kGradThreads) write_piece<T>(a, g, row, dx, piece);
+        return;
+    }
+    const float2 minus = make_float2(-g.m, -g.m), c2 = make_float2(g.c, g.c), A2 = make_float2(g.A, g.A), B2 = make_float2(g.B, g.B);
+    const float f = -a.scale * g.inv_S * (g.B != 0.f ? 1.f : g.A);
+    const float2 f2 = make_float2(f, f);
+    auto whole = [&](auto with_d) {
+        for (int base = q0 + threadIdx.x; base < q1; base += kGradTurn * kGradThreads) {
+            Piece<T, VEC> w[kGradTurn];
+#pragma unroll
+            for (int u = 0; u < kGradTurn; ++u)
+                if (base + u * kGradThreads < q1) w[u] = *(const Piece<T, VEC>*)(row.x + row.first(base + u * kGradThreads));
+#pragma unroll
+            for (int u = 0; u < kGradTurn; ++u) {
+                if (base + u * kGradThreads >= q1) break;
+                float v[VEC];
+                as_floats(w[u], v);
+                Piece<T, VEC> q;
+#pragma unroll
+                for (int k = 0; k < VEC; k += 2) {
+                    float2 d = __fmul2_rn(__fadd2_rn(make_float2(v[k], v[k + 1]), minus), c2);
+                    if (with_d) {
+                        d.x = fmaxf(d.x, kFar);
+                        d.y = fmaxf(d.y, kFar);
+                    }
+                    const float2 p = __fmul2_rn(make_float2(exp_2(d.x), exp_2(d.y)), f2);
+                    const float2 y = with_d ? __fmul2_rn(p, __ffma2_rn(B2, d, A2)) : p;
+                    q.v[k] = from_float<T>(y.x);
+                    q.v[k + 1] = from_float<T>(y.y);
+                }
+                *(Piece<T, VEC>*)(dx + row.first(base + u * kGradThreads)) = q;
+            }
+        }
+    };
+    if (g.B != 0.f) whole(std::true_type());
+    else whole(std::false_type());   // the weight is A for all
+    // the others: those that the row's ends cut, or all
+    for (int piece = p0 + threadIdx.x; piece < min(q0, p1); piece += kGradThreads) write_piece<T>(a, g, row, dx, piece);
+    for (int piece = max(q0, q1) + threadIdx.x; piece < p1; piece += kGradThreads) write_piece<T>(a, g, row, dx, piece);
     __syncthreads();   // classes with weights of their own are written once more, by one thread each (equal values where they coincide)
     for (int k = threadIdx.x; k < 1 + (a.g_top ? a.top : 0); k += kGradThreads) {
         const long long j = k ? a.top_ids[r * a.top + k - 1] : a.g_logprobs ? load_target(a.target, a.target64, r) : -1;
         if (j < 0 || j >= a.classes || (k == 0 && !target_counts(a, j))) continue;
-        const int piece = (int)((j + row.head) / Row<T>::VEC);
+        const int piece = (int)((j + row.head) / VEC);
         if (piece >= p0 && piece < p1) write_own<T>(a, r, g, row, dx, j);
     }
 }
@@ -529,6 +805,23 @@ constexpr int kShortPieces = 64 * kShortScores / Row<T>::VEC;
 template <class T>
 int most_pieces(int classes) { return (int)ceil_div64((long long)classes + Row<T>::VEC - 1, Row<T>::VEC); }
 
+template <class T, int THREADS, bool MASKED>
+int launch_rows(long long n, int parts, cudaStream_t st, const Forward& a) {
+    if (n * parts > 0x7fffffffll) return TRS_E_LIMIT;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)parts;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(n * parts));
+    cfg.blockDim = dim3(THREADS);
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = parts > 1 ? 1 : 0;
+    TRS_CUDA(cudaLaunchKernelEx(&cfg, k_row<T, THREADS, MASKED>, a, parts));
+    return TRS_OK;
+}
+
 Extent extent(const void* p, long long rows, long long stride, long long width, int size) {
     return {(uintptr_t)p, (uintptr_t)p + (size_t)((rows - 1) * stride + width) * size};
 }
@@ -565,8 +858,18 @@ extern "C" int trs_logprobs(const void* x, int type, long long n, int classes, l
                 return launch(k_short_rows<T, G, decltype(per)::value>, dim3((unsigned)ceil_div64(n * G, kShortThreads)), kShortThreads, 0,
                               (cudaStream_t)stream, a);
             });
-        if (pieces <= 256) return launch(k_row<T, 128>, dim3((unsigned)n), 128, 0, (cudaStream_t)stream, a);
-        return launch(k_row<T, 512>, dim3((unsigned)n), 512, 0, (cudaStream_t)stream, a);
+        auto run = [&](auto threads, int parts) {
+            constexpr int THREADS = decltype(threads)::value;
+            return a.mask ? launch_rows<T, THREADS, true>(n, parts, (cudaStream_t)stream, a)
+                          : launch_rows<T, THREADS, false>(n, parts, (cudaStream_t)stream, a);
+        };
+        if (pieces <= 128 * kTurn) return run(std::integral_constant<int, 128>(), 1);
+        // Few rows: parts until there are two CTAs an SM (or a part has one turn).  More of them only add ends: 512 rows of 2^18 masked
+        // fp16 scores, ten alternatives: 87 us whole, 92 / 96 / 125 us in 2 / 4 / 8 parts.
+        int parts = 1;
+        while (parts < kMaxParts && n * parts < 2 * 148 && pieces > parts * 256 * kTurn) parts *= 2;
+        if (n * parts < 2 * 148) return run(std::integral_constant<int, 512>(), parts);
+        return run(std::integral_constant<int, 256>(), parts);
     });
 }
 TRS_CATCH
@@ -594,7 +897,8 @@ extern "C" int trs_logprobs_grad(const void* x, int type, long long n, int class
             });
         const long long parts = ceil_div64((long long)classes + Row<T>::VEC - 1, (long long)Row<T>::VEC * kGradThreads * kGradPieces);
         if (n * parts > 0x7fffffffll) return (int)TRS_E_LIMIT;
-        return launch(k_row_grad<T>, dim3((unsigned)(n * parts)), kGradThreads, 0, (cudaStream_t)stream, a, (int)parts);
+        return launch(a.mask ? k_row_grad<T, true> : k_row_grad<T, false>, dim3((unsigned)(n * parts)), kGradThreads, 0, (cudaStream_t)stream, a,
+                      (int)parts);
     });
 }
 TRS_CATCH

@@ -23,6 +23,81 @@ struct alignas(sizeof(T) * N) Piece {
     T v[N];
 };
 
+// A 16-byte piece as floats.
+__device__ __forceinline__ void as_floats(const Piece<float, 4>& p, float (&v)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = p.v[k];
+}
+__device__ __forceinline__ void as_floats(const Piece<__half, 8>& p, float (&v)[8]) {
+#pragma unroll
+    for (int k = 0; k < 8; k += 2) {
+        const float2 f = __half22float2(__halves2half2(p.v[k], p.v[k + 1]));
+        v[k] = f.x;
+        v[k + 1] = f.y;
+    }
+}
+__device__ __forceinline__ void as_floats(const Piece<__nv_bfloat16, 8>& p, float (&v)[8]) {
+    const uint4 w = *(const uint4*)&p;   // bf16 is the upper half of fp32
+    const unsigned u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        v[2 * k] = __uint_as_float(u[k] << 16);
+        v[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
+    }
+}
+
+// Largest element of a piece (NaN where one is); 16-bit types two at a time.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float max_of(const Piece<float, 4>& p) { return max_nan(max_nan(p.v[0], p.v[1]), p.v[2], p.v[3]); }
+__device__ __forceinline__ float max_of(const Piece<__half, 8>& p) {
+    const __half2* h = (const __half2*)&p;
+    const float2 f = __half22float2(__hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
+    return max_nan(f.x, f.y);
+}
+__device__ __forceinline__ float max_of(const Piece<__nv_bfloat16, 8>& p) {
+    const __nv_bfloat162* h = (const __nv_bfloat162*)&p;
+    const float2 f = __bfloat1622float2(__hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
+    return max_nan(f.x, f.y);
+}
+
+// -inf where the byte of the mask is 0: `bytes` has four of them, the first for element `from` of the piece.
+__device__ __forceinline__ unsigned nonzero_bytes(unsigned bytes) {   // the top bit of every byte that is not 0 (the others as they come)
+    return ((bytes & 0x7f7f7f7fu) + 0x7f7f7f7fu) | bytes;
+}
+__device__ __forceinline__ void mask_four(Piece<float, 4>& p, int from, unsigned bytes) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (!(bytes >> (8 * k) & 0xff)) p.v[from + k] = -INFINITY;
+}
+template <unsigned SELECT>
+__device__ __forceinline__ unsigned spread(unsigned x) {   // prmt with the bytes' top bits repeated
+    unsigned r;
+    asm("prmt.b32 %0, %1, 0, %2;" : "=r"(r) : "r"(x), "n"(SELECT));
+    return r;
+}
+template <unsigned INF>
+__device__ __forceinline__ void mask_four_16(unsigned* two, unsigned bytes) {
+    const unsigned top = nonzero_bytes(bytes);
+    const unsigned lo = spread<0x9988>(top), hi = spread<0xbbaa>(top);   // top bits spread over 16 bits each
+    two[0] = (two[0] & lo) | (INF & ~lo);
+    two[1] = (two[1] & hi) | (INF & ~hi);
+}
+__device__ __forceinline__ void mask_four(Piece<__half, 8>& p, int from, unsigned bytes) {
+    mask_four_16<0xfc00fc00u>((unsigned*)&p + from / 2, bytes);
+}
+__device__ __forceinline__ void mask_four(Piece<__nv_bfloat16, 8>& p, int from, unsigned bytes) {
+    mask_four_16<0xff80ff80u>((unsigned*)&p + from / 2, bytes);
+}
+
 inline int type_bytes(int type) { return type == TRS_TYPE_F32 ? 4 : 2; }
 inline bool type_known(int type) { return type == TRS_TYPE_F32 || type == TRS_TYPE_F16 || type == TRS_TYPE_BF16; }
 
