@@ -35,25 +35,22 @@ __global__ void __launch_bounds__(kThreads) k_lookup(const TI* __restrict__ tabl
     float mul[kLookupRows];
 #pragma unroll
     for (int u = 0; u < kLookupRows; ++u) {
-        const long long id = i0 + u < n ? load_id(ids, ids64, i0 + u) : 0;
-        const bool pad = id == padding && padding != TRS_NO_PADDING, bad = id < 0 || id >= rows;
-        // no row to read: the result is the constant
-        from[u] = pad || bad || i0 + u >= n ? nullptr : table + id * stride;
-        mul[u] = pad ? 0.f : bad ? __int_as_float(0x7fffffff) : scale;
+        const long long id = i0 + u < n ? load_id(ids, ids64, i0 + u) : -1;
+        const bool pad = id == padding && padding != TRS_NO_PADDING, bad = (unsigned long long)id >= (unsigned long long)rows;
+        from[u] = pad || bad ? nullptr : table + id * stride + lane * VEC;
+        mul[u] = pad ? 0.f : bad ? __int_as_float(0x7fffffff) : scale;   // what zeros are multiplied by where there is no row
     }
+    TO* to = out + i0 * out_stride + lane * VEC;
     for (int c = lane; c < pieces; c += G) {
         Piece<TI, VEC> p[kLookupRows];
 #pragma unroll
-        for (int u = 0; u < kLookupRows; ++u)
-            if (from[u]) p[u] = *(const Piece<TI, VEC>*)(from[u] + (size_t)c * VEC);
-#pragma unroll
         for (int u = 0; u < kLookupRows; ++u) {
-            if (i0 + u >= n) break;
-            Piece<TO, VEC> q;
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) q.v[k] = from_float<TO>(from[u] ? as_float(p[u].v[k]) * mul[u] : mul[u]);
-            *(Piece<TO, VEC>*)(out + (i0 + u) * out_stride + (size_t)c * VEC) = q;
+            p[u] = Piece<TI, VEC>{};
+            if (from[u]) p[u] = *(const Piece<TI, VEC>*)(from[u] + (c - lane) * VEC);
         }
+#pragma unroll
+        for (int u = 0; u < kLookupRows; ++u)
+            if (i0 + u < n) *(Piece<TO, VEC>*)(to + u * out_stride + (c - lane) * VEC) = scaled<TO>(p[u], mul[u]);
     }
 }
 
@@ -75,15 +72,21 @@ __global__ void __launch_bounds__(kSortThreads) k_digit_counts(const void* __res
                                                                const unsigned* __restrict__ keys, int n, int shift, int digit_bits,
                                                                int* __restrict__ counts, int2* __restrict__ segment) {
     extern __shared__ int s_count[];
+    if (!FIRST) wait_for_kernel_before();
     const int bins = 1 << digit_bits, tiles = gridDim.x;
     for (int b = threadIdx.x; b < bins; b += kSortThreads) s_count[b] = 0;
     __syncthreads();
     const int base = blockIdx.x * kTile;
+    unsigned key[kSortItems];
+#pragma unroll
     for (int k = 0; k < kSortItems; ++k) {
         const int i = base + k * kSortThreads + threadIdx.x;
-        if (i >= n || i < base) break;
-        const unsigned key = FIRST ? key_of(load_id(ids, ids64, i), rows, padding) : keys[i];
-        atomicAdd(&s_count[(key >> shift) & (bins - 1)], 1);
+        if (i < n && i >= 0) key[k] = FIRST ? key_of(load_id(ids, ids64, i), rows, padding) : keys[i];
+    }
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k) {
+        const int i = base + k * kSortThreads + threadIdx.x;
+        if (i < n && i >= 0) atomicAdd(&s_count[(key[k] >> shift) & (bins - 1)], 1);
     }
     __syncthreads();
     for (int b = threadIdx.x; b < bins; b += kSortThreads) counts[(size_t)b * tiles + blockIdx.x] = s_count[b];
@@ -95,6 +98,7 @@ __global__ void __launch_bounds__(kSortThreads) k_digit_counts(const void* __res
 // counts[bin, tile] -> the number of keys with that digit in earlier tiles; total[bin].  One warp a bin.
 __global__ void __launch_bounds__(256) k_digit_prefix(int* __restrict__ counts, int tiles, int bins, int* __restrict__ total) {
     const int bin = (blockIdx.x * 256 + threadIdx.x) / 32, lane = threadIdx.x % 32;
+    wait_for_kernel_before();
     if (bin >= bins) return;
     int* c = counts + (size_t)bin * tiles;
     int sum = 0;
@@ -125,6 +129,7 @@ __global__ void __launch_bounds__(kSortThreads) k_digit_scatter(const void* __re
     unsigned short* s_rank = (unsigned short*)(s_mem + bins);       // [warps][bins]
     __shared__ int s_sum[kSortWarps];
     for (int k = threadIdx.x; k < bins * kSortWarps / 2; k += kSortThreads) ((int*)s_rank)[k] = 0;
+    wait_for_kernel_before();
     // prefix sums of the digits' totals: each thread has bins / threads neighbouring ones
     const int per = (bins + kSortThreads - 1) / kSortThreads, b0 = threadIdx.x * per;
     int mine = 0;
@@ -200,95 +205,194 @@ __device__ __forceinline__ void add_row(float (&acc)[VEC], const T* __restrict__
     for (int k = 0; k < VEC; ++k) acc[k] += as_float(p.v[k]);
 }
 
+// The sum of the 64 rows whose positions the warp's lanes hold (pa: the first 32), at piece c of a group of G lanes; the groups of the warp
+// take the positions in turn, and their sums are added in a fixed order.  All lanes come along.
+template <class T, int VEC, int G>
+__device__ __forceinline__ void sum_block(float (&acc)[VEC], const T* __restrict__ g, long long stride, int pa, int pb, int c, int pieces) {
+    constexpr int GROUPS = 32 / G;
+    const int group = threadIdx.x % 32 / G;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < kBlock / GROUPS; ++i) {
+        const int j = i * GROUPS + group, p = __shfl_sync(0xffffffffu, i < kBlock / GROUPS / 2 ? pa : pb, j % 32);
+        if (c < pieces) add_row<T, VEC>(acc, g + (size_t)p * stride, c);
+    }
+#pragma unroll
+    for (int o = G; o < 32; o *= 2)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[k] += __shfl_xor_sync(0xffffffffu, acc[k], o);
+}
+
 // One CTA a span: notes where segments begin and end, and sums its uniform blocks.
-template <class T, int VEC>
+template <class T, int VEC, int G>
 __global__ void __launch_bounds__(kThreads) k_block_sums(const T* __restrict__ g, long long stride, const unsigned* __restrict__ keys,
                                                          const int* __restrict__ pos, int n, unsigned rows, int F, int span,
                                                          int2* __restrict__ segment, float* __restrict__ block_sum,
                                                          float* __restrict__ span_sum) {
+    wait_for_kernel_before();
     const int p0 = blockIdx.x * span, p1 = min(n - p0, span) + p0;
-    for (int p = p0 + threadIdx.x; p < p1; p += kThreads) {
-        const unsigned k = keys[p];
-        if (k >= rows) continue;
-        if (p == 0 || keys[p - 1] != k) segment[k].x = p;
-        if (p == n - 1 || keys[p + 1] != k) segment[k].y = p + 1;
-    }
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, pieces = F / VEC;
     const bool whole = p1 - p0 == span && keys[p0] == keys[p1 - 1] && keys[p0] < rows;
-    __shared__ float s_part[kSpanWarps][32 * VEC];
-    for (int c0 = 0; c0 < pieces; c0 += 32) {
-        const int c = c0 + lane;
+    for (int b = p0 + warp * kBlock; b < p1; b += kSpanWarps * kBlock) {
+        const int i0 = b + lane, i1 = i0 + 32;
+        const unsigned none = ~0u, k0 = i0 < n ? keys[i0] : none, k1 = i1 < n ? keys[i1] : none;
+        unsigned edge = none;   // the keys around the block
+        if (lane == 0 && b > 0) edge = keys[b - 1];
+        if (lane == 31 && b + kBlock < n) edge = keys[b + kBlock];
+        const unsigned k0_up = __shfl_up_sync(none, k0, 1), k1_up = __shfl_up_sync(none, k1, 1), k0_down = __shfl_down_sync(none, k0, 1),
+                       k1_down = __shfl_down_sync(none, k1, 1), k0_last = __shfl_sync(none, k0, 31), k1_first = __shfl_sync(none, k1, 0);
+        auto note = [&](int i, unsigned k, unsigned before, unsigned after) {
+            if (k >= rows) return;
+            if (before != k && after != k) segment[k] = make_int2(i, i + 1);
+            else if (before != k) segment[k].x = i;
+            else if (after != k) segment[k].y = i + 1;
+        };
+        note(i0, k0, lane ? k0_up : edge, lane < 31 ? k0_down : k1_first);
+        note(i1, k1, lane ? k1_up : k0_last, lane < 31 ? k1_down : edge);
+        if (whole) continue;
+        const unsigned key = __shfl_sync(none, k0, 0);
+        if (!__all_sync(none, k0 == key && k1 == key) || key >= rows) continue;   // (the end of the list is not: none)
+        const int pa = pos[i0], pb = pos[i1];
+        for (int c0 = 0; c0 < pieces; c0 += G) {
+            const int c = c0 + lane % G;
+            float acc[VEC];
+            sum_block<T, VEC, G>(acc, g, stride, pa, pb, c, pieces);
+            if (c < pieces && lane < G)
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) block_sum[(size_t)(b / kBlock) * F + c * VEC + k] = acc[k];
+        }
+    }
+    if (!whole) return;   // the same for all threads of the CTA
+    __shared__ float s_part[kSpanWarps][G * VEC];
+    for (int c0 = 0; c0 < pieces; c0 += G) {
+        const int c = c0 + lane % G;
         float sum[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; ++k) sum[k] = 0.f;
-        for (int b = p0 + warp * kBlock; b + kBlock <= p1; b += kSpanWarps * kBlock) {
-            if (!whole && (keys[b] != keys[b + kBlock - 1] || keys[b] >= rows)) continue;
+        for (int b = p0 + warp * kBlock; b < p1; b += kSpanWarps * kBlock) {
             float acc[VEC];
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
-            if (c < pieces) {
-#pragma unroll 8
-                for (int p = b; p < b + kBlock; ++p) add_row<T, VEC>(acc, g + (size_t)pos[p] * stride, c);
-                if (!whole)
-#pragma unroll
-                    for (int k = 0; k < VEC; ++k) block_sum[(size_t)(b / kBlock) * F + c * VEC + k] = acc[k];
-            }
+            sum_block<T, VEC, G>(acc, g, stride, pos[b + lane], pos[b + 32 + lane], c, pieces);
 #pragma unroll
             for (int k = 0; k < VEC; ++k) sum[k] += acc[k];
         }
-        if (whole) {   // the same for all threads of the CTA
-            __syncthreads();
+        __syncthreads();
+        if (lane < G)
 #pragma unroll
             for (int k = 0; k < VEC; ++k) s_part[warp][lane * VEC + k] = sum[k];
-            __syncthreads();
-            for (int f = threadIdx.x; f < 32 * VEC; f += kThreads) {
-                float s = 0.f;
-                for (int w = 0; w < kSpanWarps; ++w) s += s_part[w][f];
-                if (c0 * VEC + f < F) span_sum[(size_t)blockIdx.x * F + c0 * VEC + f] = s;
-            }
+        __syncthreads();
+        for (int f = threadIdx.x; f < G * VEC; f += kThreads) {
+            float s = 0.f;
+            for (int w = 0; w < kSpanWarps; ++w) s += s_part[w][f];
+            if (c0 * VEC + f < F) span_sum[(size_t)blockIdx.x * F + c0 * VEC + f] = s;
         }
     }
 }
 
-// A group of G lanes sums one row's segment for G pieces of the row.
+// A group of G lanes sums the segments of kSumRows neighbouring rows for G pieces of the row: first those of up to kSumAhead positions,
+// all together (most rows have no more where ids are spread), then the others one by one, kSumBatch positions at a time.
+constexpr int kSumRows = 4, kSumAhead = 2, kSumBatch = 8, kPartBatch = 4;
+
+template <class TO, int VEC>
+__device__ __forceinline__ void write_sum(TO* __restrict__ o, const float (&acc)[VEC], float scale, int accumulate) {
+    Piece<TO, VEC> q;
+    if (accumulate) q = *(Piece<TO, VEC>*)o;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) q.v[k] = from_float<TO>(accumulate ? fmaf(scale, acc[k], as_float(q.v[k])) : scale * acc[k]);
+    *(Piece<TO, VEC>*)o = q;
+}
+
 template <class TI, class TO, int VEC, int G>
 __global__ void __launch_bounds__(kThreads) k_sums(const TI* __restrict__ g, long long stride, const int* __restrict__ pos, int n,
                                                    long long rows, int F, int slabs, int span, const int2* __restrict__ segment,
                                                    const float* __restrict__ block_sum, const float* __restrict__ span_sum, float scale,
                                                    TO* __restrict__ out, long long out_stride, int accumulate) {
-    const long long item = ((long long)blockIdx.x * kThreads + threadIdx.x) / G;
-    const long long v = slabs == 1 ? item : item / slabs;
-    const int c = (slabs == 1 ? 0 : (int)(item - v * slabs) * G) + threadIdx.x % G;
-    if (v >= rows || c >= F / VEC) return;
-    int p = 0, end = 0;
-    if (n > 0) {
-        const int2 s = segment[v];
-        p = s.x;
-        end = s.y;
-    }
-    if (accumulate && p == end) return;
-    float acc[VEC];
+    wait_for_kernel_before();
+    const long long item = ((long long)blockIdx.x * kThreads + threadIdx.x) / G, four = slabs == 1 ? item : item / slabs;
+    const long long v0 = four * kSumRows;
+    const int c = (slabs == 1 ? 0 : (int)(item - four * slabs) * G) + threadIdx.x % G;
+    if (v0 >= rows || c >= F / VEC) return;
+    g += (size_t)c * VEC;
+    out += v0 * out_stride + (size_t)c * VEC;
+    bool more = false;
+    {
+        int at[kSumRows][kSumAhead];
+        bool here[kSumRows];
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
-    while (p < end) {
-        if ((p & (kBlock - 1)) == 0 && p + kBlock <= end) {
-            const bool whole = p % span == 0 && p + span <= end;
-            const float* from = whole ? span_sum + (size_t)(p / span) * F : block_sum + (size_t)(p / kBlock) * F;
+        for (int u = 0; u < kSumRows; ++u) {
+            const int2 s = n > 0 && v0 + u < rows ? segment[v0 + u] : make_int2(0, 0);
+            const int count = s.y - s.x;
+            here[u] = v0 + u < rows && count <= kSumAhead && !(accumulate && count == 0);
+            more |= count > kSumAhead;
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) acc[k] += from[c * VEC + k];
-            p += whole ? span : kBlock;
-        } else {
-            const int stop = min(end, (p & ~(kBlock - 1)) + kBlock);
-#pragma unroll 4
-            for (; p < stop; ++p) add_row<TI, VEC>(acc, g + (size_t)pos[p] * stride, c);
+            for (int k = 0; k < kSumAhead; ++k) at[u][k] = here[u] && k < count ? pos[s.x + k] : -1;
+        }
+        Piece<TI, VEC> first[kSumRows][kSumAhead];
+#pragma unroll
+        for (int u = 0; u < kSumRows; ++u)
+#pragma unroll
+            for (int k = 0; k < kSumAhead; ++k) {
+                first[u][k] = Piece<TI, VEC>{};
+                if (at[u][k] >= 0) first[u][k] = *(const Piece<TI, VEC>*)(g + (size_t)at[u][k] * stride);
+            }
+#pragma unroll
+        for (int u = 0; u < kSumRows; ++u) {
+            if (!here[u]) continue;
+            float acc[VEC];
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) acc[k] = as_float(first[u][0].v[k]) + as_float(first[u][1].v[k]);
+            write_sum<TO, VEC>(out + u * out_stride, acc, scale, accumulate);
         }
     }
-    TO* o = out + v * out_stride + (size_t)c * VEC;
-    Piece<TO, VEC> q;
-    if (accumulate) q = *(Piece<TO, VEC>*)o;
+    if (!more) return;
+#pragma unroll 1
+    for (int u = 0; u < kSumRows; ++u) {
+        if (v0 + u >= rows) break;
+        const int2 s = segment[v0 + u];
+        int p = s.x;
+        const int end = s.y;
+        if (end - p <= kSumAhead) continue;
+        float acc[VEC];
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) q.v[k] = from_float<TO>(accumulate ? as_float(q.v[k]) + scale * acc[k] : scale * acc[k]);
-    *(Piece<TO, VEC>*)o = q;
+        for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+        while (p < end) {
+            // whole blocks and spans from their sums, single positions otherwise
+            if ((p & (kBlock - 1)) == 0 && p + kBlock <= end) {
+                const bool spans = p % span == 0 && p + span <= end;
+                const int step = spans ? span : kBlock;
+                const float* from = (spans ? span_sum + (size_t)(p / span) * F : block_sum + (size_t)(p / kBlock) * F) + c * VEC;
+                // blocks up to the next span (which is taken as one) or the segment's end
+                const int stop = spans ? end : min(end, p - p % span + span), count = min((stop - p) / step, kPartBatch);
+                Piece<float, VEC> part[kPartBatch];
+#pragma unroll
+                for (int k = 0; k < kPartBatch; ++k)
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) part[k].v[q] = k < count ? from[(size_t)k * F + q] : 0.f;
+#pragma unroll
+                for (int k = 0; k < kPartBatch; ++k)
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) acc[q] += part[k].v[q];
+                p += count * step;
+            } else {
+                const int stop = min(end, (p & ~(kBlock - 1)) + kBlock);
+                Piece<TI, VEC> row[kSumBatch];
+                int at[kSumBatch];
+#pragma unroll
+                for (int k = 0; k < kSumBatch; ++k) at[k] = p + k < stop ? pos[p + k] : -1;
+#pragma unroll
+                for (int k = 0; k < kSumBatch; ++k) {
+                    row[k] = Piece<TI, VEC>{};
+                    if (at[k] >= 0) row[k] = *(const Piece<TI, VEC>*)(g + (size_t)at[k] * stride);
+                }
+#pragma unroll
+                for (int k = 0; k < kSumBatch; ++k)
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) acc[q] += as_float(row[k].v[q]);
+                p = min(p + kSumBatch, stop);
+            }
+        }
+        write_sum<TO, VEC>(out + u * out_stride, acc, scale, accumulate);
+    }
 }
 
 // ----------------------------------------------------------------------------------------------
@@ -337,9 +441,9 @@ GradPlan grad_plan(long long n, long long rows, int F) {
     p.digits = (bits + kMaxDigit - 1) / kMaxDigit;
     p.digit_bits = (bits + p.digits - 1) / p.digits;
     p.tiles = (int)ceil_div64(n, kTile);
-    // spans: some 600 of them, of 512 to 8192 positions
+    // spans: up to about a thousand of them, of 512 positions or more
     p.span = kBlock * kSpanWarps;
-    while (p.span < 8192 && (long long)p.span * 592 < n) p.span *= 2;
+    while (p.span < (1 << 20) && (long long)p.span * 1024 < n) p.span *= 2;
     p.spans = (int)ceil_div64(n, p.span);
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -375,15 +479,15 @@ int sort_pass(const void* ids, int ids64, long long rows, long long padding, uns
     const unsigned* keys = (const unsigned*)(ws + p.keys[from]);
     const int* pos = (const int*)(ws + p.pos[from]);
     int *counts = (int*)(ws + p.counts), *total = (int*)(ws + p.total);
-    int rc = launch(k_digit_counts<FIRST>, dim3(p.tiles), kSortThreads, (size_t)bins * 4, st, ids, ids64, rows, padding, keys, n, shift,
+    int rc = launch_behind(k_digit_counts<FIRST>, dim3(p.tiles), kSortThreads, (size_t)bins * 4, st, !FIRST, ids, ids64, rows, padding, keys, n, shift,
                     p.digit_bits, counts, (int2*)(ws + p.segment));
     if (rc) return rc;
-    rc = launch(k_digit_prefix, dim3(ceil_div(bins, 8)), 256, 0, st, counts, p.tiles, bins, total);
+    rc = launch_behind(k_digit_prefix, dim3(ceil_div(bins, 8)), 256, 0, st, true, counts, p.tiles, bins, total);
     if (rc) return rc;
     const size_t smem = (size_t)bins * (4 + 2 * kSortWarps);
     rc = allow_smem(k_digit_scatter<FIRST>, (1 << kMaxDigit) * (4 + 2 * kSortWarps), false, g_scatter_done[FIRST]);
     if (rc) return rc;
-    return launch(k_digit_scatter<FIRST>, dim3(p.tiles), kSortThreads, smem, st, ids, ids64, rows, padding, keys, pos, n, shift, p.digit_bits,
+    return launch_behind(k_digit_scatter<FIRST>, dim3(p.tiles), kSortThreads, smem, st, true, ids, ids64, rows, padding, keys, pos, n, shift, p.digit_bits,
                   (const int*)counts, (const int*)total, (unsigned*)(ws + p.keys[to]), (int*)(ws + p.pos[to]));
 }
 
@@ -466,26 +570,26 @@ extern "C" int trs_embedding_grad(const void* grad, int grad_type, long long gra
             if constexpr (VEC * sizeof(TI) > 16) {
                 return (int)TRS_E_ARG;   // not reached: elements_per_piece
             } else {
-                if (n) {
-                    const int e = launch(k_block_sums<TI, VEC>, dim3(p.spans), kThreads, 0, st, (const TI*)grad, grad_stride, keys, pos, (int)n,
-                                         (unsigned)rows, F, p.span, segment, block_sum, span_sum);
-                    if (e) return e;
-                }
-                return with_type(out_type, [&](auto to) {
-                    using TO = decltype(to);
-                    if constexpr (VEC * sizeof(TO) > 16) {
-                        return (int)TRS_E_ARG;   // not reached: elements_per_piece
-                    } else {
-                        return with_group(pieces, [&](auto gr) {
-                            constexpr int G = decltype(gr)::value;
-                            const int slabs = ceil_div(pieces, G);
-                            const long long threads = rows * slabs * G;
-                            if (ceil_div64(threads, kThreads) > 0x7fffffffll) return (int)TRS_E_LIMIT;
-                            return launch(k_sums<TI, TO, VEC, G>, dim3((unsigned)ceil_div64(threads, kThreads)), kThreads, 0, st,
-                                          (const TI*)grad, grad_stride, pos, (int)n, rows, F, slabs, p.span, (const int2*)segment,
-                                          (const float*)block_sum, (const float*)span_sum, scale, (TO*)out, out_stride, accumulate);
-                        });
+                return with_group(pieces, [&](auto gr) {
+                    constexpr int G = decltype(gr)::value;
+                    if (n) {
+                        const int e = launch_behind(k_block_sums<TI, VEC, G>, dim3(p.spans), kThreads, 0, st, true, (const TI*)grad, grad_stride, keys, pos,
+                                                    (int)n, (unsigned)rows, F, p.span, segment, block_sum, span_sum);
+                        if (e) return e;
                     }
+                    return with_type(out_type, [&](auto to) {
+                        using TO = decltype(to);
+                        if constexpr (VEC * sizeof(TO) > 16) {
+                            return (int)TRS_E_ARG;   // not reached: elements_per_piece
+                        } else {
+                            const int slabs = ceil_div(pieces, G);
+                            const long long threads = ceil_div64(rows, kSumRows) * slabs * G;
+                            if (ceil_div64(threads, kThreads) > 0x7fffffffll) return (int)TRS_E_LIMIT;
+                            return launch_behind(k_sums<TI, TO, VEC, G>, dim3((unsigned)ceil_div64(threads, kThreads)), kThreads, 0, st, n > 0,
+                                                 (const TI*)grad, grad_stride, pos, (int)n, rows, F, slabs, p.span, (const int2*)segment,
+                                                 (const float*)block_sum, (const float*)span_sum, scale, (TO*)out, out_stride, accumulate);
+                        }
+                    });
                 });
             }
         });

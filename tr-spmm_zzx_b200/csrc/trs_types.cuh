@@ -4,6 +4,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "trs_common.cuh"
 
 namespace trs {
@@ -44,6 +46,28 @@ __device__ __forceinline__ void as_floats(const Piece<__nv_bfloat16, 8>& p, floa
         v[2 * k] = __uint_as_float(u[k] << 16);
         v[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
     }
+}
+
+// x times a factor, in fp32, rounded once: pieces of N elements, two at a time.
+template <class TO, class TI, int N>
+__device__ __forceinline__ Piece<TO, N> scaled(const Piece<TI, N>& p, float mul) {
+    Piece<TO, N> q;
+    if constexpr (N >= 2) {
+#pragma unroll
+        for (int k = 0; k < N; k += 2) {
+            float2 v;
+            if constexpr (sizeof(TI) == 4) v = make_float2(p.v[k], p.v[k + 1]);
+            else if constexpr (std::is_same<TI, __half>::value) v = __half22float2(__halves2half2(p.v[k], p.v[k + 1]));
+            else v = __bfloat1622float2(__halves2bfloat162(p.v[k], p.v[k + 1]));
+            v = __fmul2_rn(v, make_float2(mul, mul));
+            if constexpr (std::is_same<TO, __half>::value) *(__half2*)&q.v[k] = __float22half2_rn(v);
+            else if constexpr (std::is_same<TO, __nv_bfloat16>::value) *(__nv_bfloat162*)&q.v[k] = __float22bfloat162_rn(v);
+            else q.v[k] = v.x, q.v[k + 1] = v.y;
+        }
+    } else {
+        q.v[0] = from_float<TO>(as_float(p.v[0]) * mul);
+    }
+    return q;
 }
 
 // Largest element of a piece (NaN where one is); 16-bit types two at a time.
