@@ -190,6 +190,45 @@ __global__ void __launch_bounds__(kSortThreads) k_digit_scatter(const void* __re
     }
 }
 
+// Up to kFewIds ids: one CTA sorts (key, position) words in shared memory by a bitonic network, the other CTAs empty the segments.
+// (4 K ids of a 16 K row table by the digit passes: six launches, 25 us of them; this one 5 us.)
+constexpr int kFewIds = 4096, kFewThreads = 1024;
+
+__global__ void __launch_bounds__(kFewThreads) k_sort_few(const void* __restrict__ ids, int ids64, long long rows, long long padding, int n,
+                                                          int size, unsigned* __restrict__ keys_out, int* __restrict__ pos_out,
+                                                          int2* __restrict__ segment) {
+    const int threads = blockDim.x;   // up to half of `size`, the power of two from 64 on that holds n
+    if (blockIdx.x) {
+        for (long long v = (long long)(blockIdx.x - 1) * threads + threadIdx.x; v < rows; v += (long long)(gridDim.x - 1) * threads)
+            segment[v] = make_int2(0, 0);
+        return;
+    }
+    __shared__ unsigned long long s_word[kFewIds];
+    for (int i = threadIdx.x; i < size; i += threads)
+        s_word[i] = i < n ? (unsigned long long)key_of(load_id(ids, ids64, i), rows, padding) << 32 | (unsigned)i : ~0ull;
+    __syncthreads();
+    for (int run = 2; run <= size; run *= 2) {
+        for (int o = run / 2; o; o /= 2) {
+            for (int i = threadIdx.x; i < size / 2; i += threads) {
+                const int lo = 2 * i - (i & (o - 1)), hi = lo + o;
+                const unsigned long long a = s_word[lo], b = s_word[hi];
+                if ((a > b) == ((lo & run) == 0)) {
+                    s_word[lo] = b;
+                    s_word[hi] = a;
+                }
+            }
+            // 32 neighbouring pairs of a distance up to 32 are 64 words of their own
+            if (o > 32 || (o == 1 && run >= 64)) __syncthreads();
+            else __syncwarp();
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += threads) {
+        keys_out[i] = (unsigned)(s_word[i] >> 32);
+        pos_out[i] = (int)(unsigned)s_word[i];
+    }
+}
+
 // ----------------------------------------------------------------------------------------------
 // Sums of equal ids
 // ----------------------------------------------------------------------------------------------
@@ -200,9 +239,7 @@ constexpr int kBlock = 64, kSpanWarps = kThreads / 32;
 
 template <class T, int VEC>
 __device__ __forceinline__ void add_row(float (&acc)[VEC], const T* __restrict__ row, int c) {
-    const Piece<T, VEC> p = *(const Piece<T, VEC>*)(row + (size_t)c * VEC);
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) acc[k] += as_float(p.v[k]);
+    add_piece(acc, *(const Piece<T, VEC>*)(row + (size_t)c * VEC));
 }
 
 // The sum of the 64 rows whose positions the warp's lanes hold (pa: the first 32), at piece c of a group of G lanes; the groups of the warp
@@ -289,9 +326,10 @@ __global__ void __launch_bounds__(kThreads) k_block_sums(const T* __restrict__ g
     }
 }
 
-// A group of G lanes sums the segments of kSumRows neighbouring rows for G pieces of the row: first those of up to kSumAhead positions,
-// all together (most rows have no more where ids are spread), then the others one by one, kSumBatch positions at a time.
-constexpr int kSumRows = 4, kSumAhead = 2, kSumBatch = 8, kPartBatch = 4;
+// A group of G lanes writes kSumRows neighbouring rows, G pieces of each.  Their positions are neighbours too: where no row has a block's
+// worth of them, the group streams through them, kSumBatch at a time, and writes a row when the key changes; otherwise it goes
+// row by row and takes the blocks' and spans' sums.
+constexpr int kSumRows = 8, kSumBatch = 8, kPartBatch = 4;
 
 template <class TO, int VEC>
 __device__ __forceinline__ void write_sum(TO* __restrict__ o, const float (&acc)[VEC], float scale, int accumulate) {
@@ -303,55 +341,69 @@ __device__ __forceinline__ void write_sum(TO* __restrict__ o, const float (&acc)
 }
 
 template <class TI, class TO, int VEC, int G>
-__global__ void __launch_bounds__(kThreads) k_sums(const TI* __restrict__ g, long long stride, const int* __restrict__ pos, int n,
-                                                   long long rows, int F, int slabs, int span, const int2* __restrict__ segment,
-                                                   const float* __restrict__ block_sum, const float* __restrict__ span_sum, float scale,
-                                                   TO* __restrict__ out, long long out_stride, int accumulate) {
+__global__ void __launch_bounds__(kThreads) k_sums(const TI* __restrict__ g, long long stride, const unsigned* __restrict__ keys,
+                                                   const int* __restrict__ pos, int n, long long rows, int F, int slabs, int span,
+                                                   const int2* __restrict__ segment, const float* __restrict__ block_sum,
+                                                   const float* __restrict__ span_sum, float scale, TO* __restrict__ out,
+                                                   long long out_stride, int accumulate) {
     wait_for_kernel_before();
-    const long long item = ((long long)blockIdx.x * kThreads + threadIdx.x) / G, four = slabs == 1 ? item : item / slabs;
-    const long long v0 = four * kSumRows;
-    const int c = (slabs == 1 ? 0 : (int)(item - four * slabs) * G) + threadIdx.x % G;
+    const long long item = ((long long)blockIdx.x * kThreads + threadIdx.x) / G, set = slabs == 1 ? item : item / slabs;
+    const long long v0 = set * kSumRows;
+    const int c = (slabs == 1 ? 0 : (int)(item - set * slabs) * G) + threadIdx.x % G;
     if (v0 >= rows || c >= F / VEC) return;
     g += (size_t)c * VEC;
     out += v0 * out_stride + (size_t)c * VEC;
-    bool more = false;
+    int begin = n, end_all = 0;
+    bool blocks = false;
     {
-        int at[kSumRows][kSumAhead];
-        bool here[kSumRows];
+        int2 s[kSumRows];
+#pragma unroll
+        for (int u = 0; u < kSumRows; ++u) s[u] = n > 0 && v0 + u < rows ? segment[v0 + u] : make_int2(0, 0);
 #pragma unroll
         for (int u = 0; u < kSumRows; ++u) {
-            const int2 s = n > 0 && v0 + u < rows ? segment[v0 + u] : make_int2(0, 0);
-            const int count = s.y - s.x;
-            here[u] = v0 + u < rows && count <= kSumAhead && !(accumulate && count == 0);
-            more |= count > kSumAhead;
-#pragma unroll
-            for (int k = 0; k < kSumAhead; ++k) at[u][k] = here[u] && k < count ? pos[s.x + k] : -1;
-        }
-        Piece<TI, VEC> first[kSumRows][kSumAhead];
-#pragma unroll
-        for (int u = 0; u < kSumRows; ++u)
-#pragma unroll
-            for (int k = 0; k < kSumAhead; ++k) {
-                first[u][k] = Piece<TI, VEC>{};
-                if (at[u][k] >= 0) first[u][k] = *(const Piece<TI, VEC>*)(g + (size_t)at[u][k] * stride);
+            if (s[u].x < s[u].y) {
+                begin = min(begin, s[u].x);
+                end_all = max(end_all, s[u].y);
+                blocks |= s[u].y - s[u].x >= kBlock;
+            } else if (!accumulate && v0 + u < rows) {
+                *(Piece<TO, VEC>*)(out + u * out_stride) = Piece<TO, VEC>{};
             }
-#pragma unroll
-        for (int u = 0; u < kSumRows; ++u) {
-            if (!here[u]) continue;
-            float acc[VEC];
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) acc[k] = as_float(first[u][0].v[k]) + as_float(first[u][1].v[k]);
-            write_sum<TO, VEC>(out + u * out_stride, acc, scale, accumulate);
         }
     }
-    if (!more) return;
+    if (!blocks) {
+        float acc[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+        for (int p = begin; p < end_all; p += kSumBatch) {
+            int at[kSumBatch];
+            unsigned key[kSumBatch + 1];
+#pragma unroll
+            for (int k = 0; k < kSumBatch; ++k) at[k] = p + k < end_all ? pos[p + k] : -1;
+#pragma unroll
+            for (int k = 0; k <= kSumBatch; ++k) key[k] = p + k < end_all ? keys[p + k] : ~0u;
+            Piece<TI, VEC> row[kSumBatch];
+#pragma unroll
+            for (int k = 0; k < kSumBatch; ++k)
+                if (at[k] >= 0) row[k] = *(const Piece<TI, VEC>*)(g + (size_t)at[k] * stride);
+#pragma unroll
+            for (int k = 0; k < kSumBatch; ++k) {
+                if (at[k] < 0) break;
+                add_piece(acc, row[k]);
+                if (key[k] == key[k + 1]) continue;
+                write_sum<TO, VEC>(out + (long long)(key[k] - (unsigned)v0) * out_stride, acc, scale, accumulate);
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) acc[q] = 0.f;
+            }
+        }
+        return;
+    }
 #pragma unroll 1
     for (int u = 0; u < kSumRows; ++u) {
         if (v0 + u >= rows) break;
         const int2 s = segment[v0 + u];
         int p = s.x;
         const int end = s.y;
-        if (end - p <= kSumAhead) continue;
+        if (p == end) continue;
         float acc[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
@@ -385,9 +437,7 @@ __global__ void __launch_bounds__(kThreads) k_sums(const TI* __restrict__ g, lon
                     if (at[k] >= 0) row[k] = *(const Piece<TI, VEC>*)(g + (size_t)at[k] * stride);
                 }
 #pragma unroll
-                for (int k = 0; k < kSumBatch; ++k)
-#pragma unroll
-                    for (int q = 0; q < VEC; ++q) acc[q] += as_float(row[k].v[q]);
+                for (int k = 0; k < kSumBatch; ++k) add_piece(acc, row[k]);
                 p = min(p + kSumBatch, stop);
             }
         }
@@ -551,7 +601,16 @@ extern "C" int trs_embedding_grad(const void* grad, int grad_type, long long gra
     if (n) {
         p = grad_plan(n, rows, F);
         if (!ws || workspace_bytes < p.bytes || (uintptr_t)ws % 16) return TRS_E_WORKSPACE;
-        for (int pass = 0; pass < p.digits; ++pass) {
+        if (n <= kFewIds) {
+            p.digits = 1;   // (the result is where a first pass leaves it)
+            int size = 64;
+            while (size < n) size *= 2;
+            const int threads = size / 2 < kFewThreads ? size / 2 : kFewThreads;
+            const long long zero = ceil_div64(rows, 4 * threads);
+            rc = launch(k_sort_few, dim3(1 + (unsigned)(zero < 2 * 148 ? zero : 2 * 148)), threads, 0, st, ids, ids64, rows, padding_id, (int)n, size, (unsigned*)(ws + p.keys[0]),
+                        (int*)(ws + p.pos[0]), (int2*)(ws + p.segment));
+            if (rc) return rc;
+        } else for (int pass = 0; pass < p.digits; ++pass) {
             rc = pass == 0 ? sort_pass<true>(ids, ids64, rows, padding_id, ws, p, (int)n, pass, st)
                            : sort_pass<false>(ids, ids64, rows, padding_id, ws, p, (int)n, pass, st);
             if (rc) return rc;
@@ -586,7 +645,7 @@ extern "C" int trs_embedding_grad(const void* grad, int grad_type, long long gra
                             const long long threads = ceil_div64(rows, kSumRows) * slabs * G;
                             if (ceil_div64(threads, kThreads) > 0x7fffffffll) return (int)TRS_E_LIMIT;
                             return launch_behind(k_sums<TI, TO, VEC, G>, dim3((unsigned)ceil_div64(threads, kThreads)), kThreads, 0, st, n > 0,
-                                                 (const TI*)grad, grad_stride, pos, (int)n, rows, F, slabs, p.span, (const int2*)segment,
+                                                 (const TI*)grad, grad_stride, keys, pos, (int)n, rows, F, slabs, p.span, (const int2*)segment,
                                                  (const float*)block_sum, (const float*)span_sum, scale, (TO*)out, out_stride, accumulate);
                         }
                     });

@@ -48,6 +48,27 @@ __device__ __forceinline__ void as_floats(const Piece<__nv_bfloat16, 8>& p, floa
     }
 }
 
+// Elements k and k + 1 of a piece.
+template <class T, int N>
+__device__ __forceinline__ float2 two_of(const Piece<T, N>& p, int k) {
+    if constexpr (sizeof(T) == 4) return make_float2(p.v[k], p.v[k + 1]);
+    else if constexpr (std::is_same<T, __half>::value) return __half22float2(__halves2half2(p.v[k], p.v[k + 1]));
+    else return __bfloat1622float2(__halves2bfloat162(p.v[k], p.v[k + 1]));
+}
+template <class T, int N>
+__device__ __forceinline__ void add_piece(float (&acc)[N], const Piece<T, N>& p) {
+    if constexpr (N >= 2) {
+#pragma unroll
+        for (int k = 0; k < N; k += 2) {
+            const float2 s = __fadd2_rn(make_float2(acc[k], acc[k + 1]), two_of(p, k));
+            acc[k] = s.x;
+            acc[k + 1] = s.y;
+        }
+    } else {
+        acc[0] += as_float(p.v[0]);
+    }
+}
+
 // x times a factor, in fp32, rounded once: pieces of N elements, two at a time.
 template <class TO, class TI, int N>
 __device__ __forceinline__ Piece<TO, N> scaled(const Piece<TI, N>& p, float mul) {
@@ -55,11 +76,7 @@ __device__ __forceinline__ Piece<TO, N> scaled(const Piece<TI, N>& p, float mul)
     if constexpr (N >= 2) {
 #pragma unroll
         for (int k = 0; k < N; k += 2) {
-            float2 v;
-            if constexpr (sizeof(TI) == 4) v = make_float2(p.v[k], p.v[k + 1]);
-            else if constexpr (std::is_same<TI, __half>::value) v = __half22float2(__halves2half2(p.v[k], p.v[k + 1]));
-            else v = __bfloat1622float2(__halves2bfloat162(p.v[k], p.v[k + 1]));
-            v = __fmul2_rn(v, make_float2(mul, mul));
+            const float2 v = __fmul2_rn(two_of(p, k), make_float2(mul, mul));
             if constexpr (std::is_same<TO, __half>::value) *(__half2*)&q.v[k] = __float22half2_rn(v);
             else if constexpr (std::is_same<TO, __nv_bfloat16>::value) *(__nv_bfloat162*)&q.v[k] = __float22bfloat162_rn(v);
             else q.v[k] = v.x, q.v[k + 1] = v.y;

@@ -33,11 +33,13 @@ def _row_stride(t: torch.Tensor, what: str) -> int:
     return max(t.stride(0), F)
 
 
-def _check_ids(ids: torch.Tensor, index: int):
+def _check_ids(ids: torch.Tensor, index: int) -> int:
+    """1 for 64-bit ids, 0 for 32-bit ones."""
     if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
         raise TypeError("ids must be torch.int64 or torch.int32")
     if ids.get_device() != index or not ids.is_contiguous():
         raise ValueError("ids must be contiguous and on the same CUDA device")
+    return 1 if ids.dtype is torch.int64 else 0
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -55,26 +57,30 @@ def _lookup(table, ids, scale, padding_id, dtype, out):
     index = table.get_device()
     if index < 0:
         raise ValueError("embedding needs CUDA tensors (there is no CPU fallback)")
-    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
+    if table.dim() != 2 or not table.numel():
         raise ValueError("the table must be [rows, F] with at least one row and one feature")
-    _check_ids(ids, index)
+    wide = _check_ids(ids, index)
     rows, F = table.shape
-    code = _type_code(table.dtype, "the table")
+    code = out_code = _type_code(table.dtype, "the table")
+    stride, out_stride = F if table.is_contiguous() else _row_stride(table, "the table"), F
     if out is None:
-        out = table.new_empty((*ids.shape, F), dtype=dtype)
-        out_code, out_stride = _type_code(out.dtype, "the output"), F
+        if dtype is None or dtype is table.dtype:
+            out = table.new_empty((*ids.shape, F))
+        else:
+            out_code = _type_code(dtype, "the output")
+            out = table.new_empty((*ids.shape, F), dtype=dtype)
     else:
         if out.shape != (*ids.shape, F) or out.get_device() != index or dtype is not None and out.dtype is not dtype:
             raise ValueError("out must be [*ids.shape, F] of the output type on the table's device")
         out_code = _type_code(out.dtype, "the output")
-        out_stride = _row_stride(out, "out") if out.dim() == 2 else F
-        if out.dim() != 2 and not out.is_contiguous():
+        if out.dim() == 2:
+            out_stride = _row_stride(out, "out")
+        elif not out.is_contiguous():
             raise ValueError("out must be contiguous unless ids is a vector")
         if _overlap(out, table) or _overlap(out, ids):
             raise ValueError("out may not overlap the table or the ids")
-    _lib.launch(index, _lib.load().trs_embedding, table.data_ptr(), code, rows, _row_stride(table, "the table"), ids.data_ptr(),
-                1 if ids.dtype is torch.int64 else 0, ids.numel(), F, scale, _NO_PADDING if padding_id is None else padding_id,
-                out.data_ptr(), out_code, out_stride)
+    _lib.launch(index, _lib.load().trs_embedding, table.data_ptr(), code, rows, stride, ids.data_ptr(), wide, ids.numel(), F, scale,
+                _NO_PADDING if padding_id is None else padding_id, out.data_ptr(), out_code, out_stride)
     return out
 
 
@@ -86,10 +92,13 @@ class _EmbeddingFn(torch.autograd.Function):
         return _lookup(table, ids, scale, padding_id, dtype, None)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
+        if torch.is_grad_enabled():   # under create_graph
+            return _EmbeddingFn.once(ctx, dout)
         rows, scale, padding_id, dtype = ctx.args
         return embedding_grad(dout.contiguous(), ctx.saved_tensors[0], rows, scale, padding_id, dtype), None, None, None, None
+
+    once = torch.autograd.function.once_differentiable(lambda ctx, dout: _EmbeddingFn.backward(ctx, dout))
 
 
 def embedding(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, padding_id: int | None = None,
@@ -101,7 +110,7 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, paddin
     the fp16 features that the SpMM takes without a copy of the table.  `out` may be given instead (for a vector of ids its rows
     may lie apart).  Differentiable in the table where no `out` is given: the gradient is embedding_grad's, dense, in the
     table's type."""
-    if torch.is_grad_enabled() and table.requires_grad:
+    if table.requires_grad and torch.is_grad_enabled():
         if out is not None:
             raise ValueError("embedding with out= is not differentiable: call it under torch.no_grad()")
         return _EmbeddingFn.apply(table, ids, scale, padding_id, out_dtype)
@@ -121,31 +130,34 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: fl
     index = grad.get_device()
     if index < 0:
         raise ValueError("embedding_grad needs CUDA tensors (there is no CPU fallback)")
-    _check_ids(ids, index)
+    wide = _check_ids(ids, index)
     if grad.dim() < 1 or grad.shape[:-1] != ids.shape or grad.shape[-1] < 1 or n_rows < 1:
         raise ValueError("grad must be [*ids.shape, F] with at least one feature, and the table have at least one row")
     F, n = grad.shape[-1], ids.numel()
-    code = _type_code(grad.dtype, "the gradient")
-    if grad.dim() == 2:
+    code = out_code = _type_code(grad.dtype, "the gradient")
+    stride = out_stride = F
+    if not grad.is_contiguous():
+        if grad.dim() != 2:
+            raise ValueError("the gradient must be contiguous unless ids is a vector")
         stride = _row_stride(grad, "the gradient")
-    elif not grad.is_contiguous():
-        raise ValueError("the gradient must be contiguous unless ids is a vector")
-    else:
-        stride = F
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs the out tensor to add to")
-        out = grad.new_empty((n_rows, F), dtype=out_dtype)
-    elif out.shape != (n_rows, F) or out.get_device() != index or out_dtype is not None and out.dtype is not out_dtype:
-        raise ValueError("out must be [n_rows, F] of the output type on the gradient's device")
-    elif _overlap(out, grad) or _overlap(out, ids):
-        raise ValueError("out may not overlap the gradient or the ids")
-    out_code = _type_code(out.dtype, "the output")
+        if out_dtype is None or out_dtype is grad.dtype:
+            out = grad.new_empty((n_rows, F))
+        else:
+            out_code = _type_code(out_dtype, "the output")
+            out = grad.new_empty((n_rows, F), dtype=out_dtype)
+    else:
+        if out.shape != (n_rows, F) or out.get_device() != index or out_dtype is not None and out.dtype is not out_dtype:
+            raise ValueError("out must be [n_rows, F] of the output type on the gradient's device")
+        if _overlap(out, grad) or _overlap(out, ids):
+            raise ValueError("out may not overlap the gradient or the ids")
+        out_code, out_stride = _type_code(out.dtype, "the output"), _row_stride(out, "out")
     lib, need = _lib.load(), C.c_size_t()
     _lib.check(lib.trs_embedding_grad_workspace_bytes(n, n_rows, F, C.byref(need)))
     # the workspace is this call's own: calls on several streams, and graphs, do not share one
     ws = grad.new_empty(need.value, dtype=torch.uint8) if need.value else None
-    _lib.launch(index, lib.trs_embedding_grad, grad.data_ptr(), code, stride, ids.data_ptr(), 1 if ids.dtype is torch.int64 else 0, n,
-                n_rows, F, scale, _NO_PADDING if padding_id is None else padding_id, out.data_ptr(), out_code,
-                _row_stride(out, "out"), 1 if accumulate else 0, None if ws is None else ws.data_ptr(), need.value)
+    _lib.launch(index, lib.trs_embedding_grad, grad.data_ptr(), code, stride, ids.data_ptr(), wide, n, n_rows, F, scale,
+                _NO_PADDING if padding_id is None else padding_id, out.data_ptr(), out_code, out_stride, 1 if accumulate else 0, None if ws is None else ws.data_ptr(), need.value)
     return out

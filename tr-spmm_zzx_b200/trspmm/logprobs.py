@@ -35,7 +35,7 @@ def _check(logits, targets, mask, scale, top):
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError("logits must be [n, classes] with at least one class")
     n, classes = logits.shape
-    stride = _row_stride(logits, "logits")
+    stride = classes if logits.is_contiguous() else _row_stride(logits, "logits")
     code = _type_code(logits.dtype, "logits")
     if targets is not None:
         if targets.dtype is not torch.int64 and targets.dtype is not torch.int32:
@@ -64,8 +64,10 @@ def _check(logits, targets, mask, scale, top):
 def _forward(logits, targets, top, mask, scale, ignore_id) -> ClassLogprobs:
     index, front, back = _check(logits, targets, mask, scale, top)
     n = logits.shape[0]
-    entropy = logits.new_empty(n, dtype=torch.float32)
-    logprobs = torch.empty_like(entropy) if targets is not None else None
+    if targets is None:
+        logprobs, entropy = None, logits.new_empty(n, dtype=torch.float32)
+    else:   # (an empty_like takes less time than an empty with a shape)
+        logprobs, entropy = torch.empty_like(targets, dtype=torch.float32), torch.empty_like(targets, dtype=torch.float32)
     stats = entropy.new_empty((n, 2))
     top_logprobs = top_ids = None
     if top:
@@ -89,8 +91,9 @@ class _LogprobsFn(torch.autograd.Function):
         return tuple(r)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g_logprobs, g_entropy, g_top, _ids, _stats):
+        if torch.is_grad_enabled():   # under create_graph
+            return _LogprobsFn.once(ctx, g_logprobs, g_entropy, g_top, _ids, _stats)
         logits, targets, mask, entropy, top_ids, stats = ctx.saved_tensors
         scale, ignore_id = ctx.args
         if g_logprobs is None and g_entropy is None and g_top is None:
@@ -99,6 +102,8 @@ class _LogprobsFn(torch.autograd.Function):
                                  *[None if g is None else g.contiguous() for g in (g_logprobs, g_entropy, g_top)],
                                  mask=mask, scale=scale, ignore_id=ignore_id)
         return dx, None, None, None, None, None
+
+    once = torch.autograd.function.once_differentiable(lambda ctx, *g: _LogprobsFn.backward(ctx, *g))
 
 
 def class_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, top: int = 0, mask: torch.Tensor | None = None,
@@ -112,7 +117,7 @@ def class_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
     Computed in fp32, results are fp32 (top_ids int32).
 
     Differentiable in the logits through logprobs, entropy and top_logprobs (not through the choice of the alternatives)."""
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if logits.requires_grad and torch.is_grad_enabled():
         return ClassLogprobs(*_LogprobsFn.apply(logits, targets, top, mask, scale, ignore_id))
     return _forward(logits, targets, top, mask, scale, ignore_id)
 
@@ -138,16 +143,19 @@ def class_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor | None, resu
                             (result.stats, (n, 2), torch.float32)):
         if t is not None and (t.dtype is not dtype or t.shape != shape or t.get_device() != index or not t.is_contiguous()):
             raise ValueError("gradients and results must be contiguous fp32 (top_ids int32) of the result's shapes on the logits' device")
+    dx_stride = logits.shape[1]
     if out is None:
         out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     elif out.shape != logits.shape or out.dtype is not logits.dtype or out.get_device() != index:
         raise ValueError("out must have the logits' shape and type and be on their device")
     elif _overlap(out, logits):
         raise ValueError("out may not overlap the logits")
+    else:
+        dx_stride = _row_stride(out, "out")
 
     def ptr(t):
         return None if t is None else t.data_ptr()
     _lib.launch(index, _lib.load().trs_logprobs_grad, *front, _NO_IGNORE if ignore_id is None else ignore_id, *back,
                 ptr(result.top_ids) if top else None, result.stats.data_ptr(), ptr(result.entropy) if g_entropy is not None else None,
-                ptr(g_logprobs), ptr(g_entropy), ptr(g_top_logprobs) if top else None, out.data_ptr(), _row_stride(out, "out"))
+                ptr(g_logprobs), ptr(g_entropy), ptr(g_top_logprobs) if top else None, out.data_ptr(), dx_stride)
     return out
