@@ -60,17 +60,24 @@ __global__ void __launch_bounds__(kThreads) k_lookup(const TI* __restrict__ tabl
 // Stable, so that a row's positions ascend.  Positions without a row (padding, outside the table) get the key `rows` and come last.
 // The keys have bits(rows) bits, sorted by up to 11 at a time: two passes for tables of up to 4 M rows.  Pass: the counts of
 // each digit in each tile, their prefix sums over the tiles, then every key to its place.
-constexpr int kSortThreads = 512, kSortWarps = kSortThreads / 32, kSortItems = 16, kTile = kSortThreads * kSortItems, kMaxDigit = 11;
+constexpr int kSortThreads = 512, kSortWarps = kSortThreads / 32, kSortItems = 8, kTile = kSortThreads * kSortItems, kMaxDigit = 11;
 
 __device__ __forceinline__ unsigned key_of(long long id, long long rows, long long padding) {
     return id == padding || id < 0 || id >= rows ? (unsigned)rows : (unsigned)id;
 }
 
+// All segments empty, and no row popular, by `threads` threads; two at a time (the array begins on a 16-byte boundary and has room for an even number).
+__device__ __forceinline__ void empty_segments(int2* __restrict__ segment, int* __restrict__ popular, long long rows, long long me,
+                                               long long threads) {
+    if (me == 0) *popular = 0;
+    for (long long v = me; v < (rows + 1) / 2; v += threads) ((int4*)segment)[v] = make_int4(0, 0, 0, 0);
+}
+
 // FIRST: keys are made from the ids (and the segments of all rows are emptied); otherwise they are the last pass's.
 template <bool FIRST>
 __global__ void __launch_bounds__(kSortThreads) k_digit_counts(const void* __restrict__ ids, int ids64, long long rows, long long padding,
-                                                               const unsigned* __restrict__ keys, int n, int shift, int digit_bits,
-                                                               int* __restrict__ counts, int2* __restrict__ segment) {
+                                                               const uint2* __restrict__ words, int n, int shift, int digit_bits,
+                                                               int* __restrict__ counts, int2* __restrict__ segment, int* __restrict__ popular) {
     extern __shared__ int s_count[];
     if (!FIRST) wait_for_kernel_before();
     const int bins = 1 << digit_bits, tiles = gridDim.x;
@@ -81,7 +88,7 @@ __global__ void __launch_bounds__(kSortThreads) k_digit_counts(const void* __res
 #pragma unroll
     for (int k = 0; k < kSortItems; ++k) {
         const int i = base + k * kSortThreads + threadIdx.x;
-        if (i < n && i >= 0) key[k] = FIRST ? key_of(load_id(ids, ids64, i), rows, padding) : keys[i];
+        if (i < n && i >= 0) key[k] = FIRST ? key_of(load_id(ids, ids64, i), rows, padding) : words[i].x;
     }
 #pragma unroll
     for (int k = 0; k < kSortItems; ++k) {
@@ -91,8 +98,7 @@ __global__ void __launch_bounds__(kSortThreads) k_digit_counts(const void* __res
     __syncthreads();
     for (int b = threadIdx.x; b < bins; b += kSortThreads) counts[(size_t)b * tiles + blockIdx.x] = s_count[b];
     if (FIRST)
-        for (long long v = (long long)blockIdx.x * kSortThreads + threadIdx.x; v < rows; v += (long long)tiles * kSortThreads)
-            segment[v] = make_int2(0, 0);
+        empty_segments(segment, popular, rows, (long long)blockIdx.x * kSortThreads + threadIdx.x, (long long)tiles * kSortThreads);
 }
 
 // counts[bin, tile] -> the number of keys with that digit in earlier tiles; total[bin].  One warp a bin.
@@ -115,52 +121,45 @@ __global__ void __launch_bounds__(256) k_digit_prefix(int* __restrict__ counts, 
     if (lane == 0) total[bin] = sum;
 }
 
-// A warp has 16 x 32 neighbouring keys of the tile and ranks them by its own counters, 32 at a time: lanes with one digit find each
-// other, the first of them counts for all.
+// A warp has kSortItems x 32 neighbouring words of the tile and ranks them by its own counters, 32 at a time: lanes with one digit find
+// each other by a vote on each bit, the first of them counts for all.  The tile is put in order in shared memory first: a store
+// of 32 scattered words takes an SM 32 cycles, and a tile's words of one digit go to neighbouring places.
 template <bool FIRST>
-__global__ void __launch_bounds__(kSortThreads) k_digit_scatter(const void* __restrict__ ids, int ids64, long long rows, long long padding,
-                                                                const unsigned* __restrict__ keys, const int* __restrict__ pos, int n,
-                                                                int shift, int digit_bits, const int* __restrict__ counts,
-                                                                const int* __restrict__ total, unsigned* __restrict__ keys_out,
-                                                                int* __restrict__ pos_out) {
-    extern __shared__ int s_mem[];
+__global__ void __launch_bounds__(kSortThreads, 2) k_digit_scatter(const void* __restrict__ ids, int ids64, long long rows, long long padding,
+                                                                const uint2* __restrict__ words, int n, int shift, int digit_bits,
+                                                                const int* __restrict__ counts, const int* __restrict__ total,
+                                                                uint2* __restrict__ words_out) {
+    extern __shared__ __align__(16) unsigned char s_mem[];
     const int bins = 1 << digit_bits, tiles = gridDim.x, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    int* s_base = s_mem;                                            // [bins] place of the tile's first key of a digit
-    unsigned short* s_rank = (unsigned short*)(s_mem + bins);       // [warps][bins]
-    __shared__ int s_sum[kSortWarps];
+    uint2* s_word = (uint2*)s_mem;                                              // [kTile]
+    int* s_to = (int*)(s_word + kTile);                                         // [bins] a digit's first place, less its first place in the tile
+    unsigned short* s_rank = (unsigned short*)(s_to + bins);                    // [warps][bins]
+    unsigned short* s_start = s_rank + kSortWarps * bins;                       // [bins] a digit's first place in the tile
+    __shared__ int s_sum[kSortWarps], s_sum_tile[kSortWarps];
     for (int k = threadIdx.x; k < bins * kSortWarps / 2; k += kSortThreads) ((int*)s_rank)[k] = 0;
     wait_for_kernel_before();
-    // prefix sums of the digits' totals: each thread has bins / threads neighbouring ones
-    const int per = (bins + kSortThreads - 1) / kSortThreads, b0 = threadIdx.x * per;
-    int mine = 0;
-    for (int b = b0; b < b0 + per && b < bins; ++b) mine += total[b];
-    int incl = mine;
-    for (int o = 1; o < 32; o *= 2) {
-        const int y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
-    }
-    if (lane == 31) s_sum[warp] = incl;
-    __syncthreads();
-    int at = incl - mine;
-    for (int w = 0; w < warp; ++w) at += s_sum[w];
-    for (int b = b0; b < b0 + per && b < bins; ++b) {
-        s_base[b] = at + counts[(size_t)b * tiles + blockIdx.x];
-        at += total[b];
-    }
-    const int first = blockIdx.x * kTile + warp * (kSortItems * 32) + lane;
-    unsigned key[kSortItems];
+    const int base = blockIdx.x * kTile, first = base + warp * (kSortItems * 32) + lane;
+    uint2 word[kSortItems];
     unsigned short rank[kSortItems];
     unsigned short* my = s_rank + warp * bins;
 #pragma unroll
     for (int k = 0; k < kSortItems; ++k) {
         const int i = first + k * 32;
-        key[k] = i < n && i >= 0 ? (FIRST ? key_of(load_id(ids, ids64, i), rows, padding) : keys[i]) : 0u;
+        word[k] = make_uint2(0, 0);
+        if (i < n && i >= 0) word[k] = FIRST ? make_uint2(key_of(load_id(ids, ids64, i), rows, padding), i) : words[i];
     }
+    __syncthreads();
+#pragma unroll
     for (int k = 0; k < kSortItems; ++k) {
         const int i = first + k * 32;
         const bool in = i < n && i >= 0;
-        const unsigned digit = in ? (key[k] >> shift) & (bins - 1) : (unsigned)bins;   // lanes past the end match each other only
-        const unsigned same = __match_any_sync(0xffffffffu, digit);
+        const unsigned digit = (word[k].x >> shift) & (bins - 1);
+        unsigned same = __ballot_sync(0xffffffffu, in);
+#pragma unroll
+        for (int b = 0; b < kMaxDigit; ++b) {
+            const unsigned vote = __ballot_sync(0xffffffffu, digit >> b & 1);   // (bits past the digit are 0 for all)
+            same &= digit >> b & 1 ? vote : ~vote;
+        }
         const int before = __popc(same & ((1u << lane) - 1));
         int r = 0;
         if (in) r = my[digit] + before;
@@ -170,23 +169,53 @@ __global__ void __launch_bounds__(kSortThreads) k_digit_scatter(const void* __re
         rank[k] = (unsigned short)r;
     }
     __syncthreads();
-    for (int b = threadIdx.x; b < bins; b += kSortThreads) {   // counters of a digit -> keys of it in the warps before
-        int sum = 0;
+    // Prefix sums over the digits, of all keys and of the tile's: each thread has bins / threads neighbouring pairs of digits (16 bits
+    // hold a tile's counts, so two digits are added in one word).  A digit's counters become the number of its keys in the warps before.
+    const int pairs = bins / 2, per = (pairs + kSortThreads - 1) / kSortThreads, b0 = threadIdx.x * per;
+    int all = 0, here = 0;
+    for (int b = b0; b < b0 + per && b < pairs; ++b) {
+        all += total[2 * b] + total[2 * b + 1];
+        unsigned sum = 0;
+#pragma unroll
         for (int w = 0; w < kSortWarps; ++w) {
-            const int x = s_rank[w * bins + b];
-            s_rank[w * bins + b] = (unsigned short)sum;
+            const unsigned x = ((unsigned*)s_rank)[w * pairs + b];
+            ((unsigned*)s_rank)[w * pairs + b] = sum;
             sum += x;
         }
+        ((unsigned*)s_start)[b] = sum;   // for the second round
+        here += (sum & 0xffff) + (sum >> 16);
+    }
+    int incl = all, incl_tile = here;
+    for (int o = 1; o < 32; o *= 2) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, o), z = __shfl_up_sync(0xffffffffu, incl_tile, o);
+        if (lane >= o) incl += y, incl_tile += z;
+    }
+    if (lane == 31) s_sum[warp] = incl, s_sum_tile[warp] = incl_tile;
+    __syncthreads();
+    int at = incl - all, at_tile = incl_tile - here;
+    for (int w = 0; w < warp; ++w) at += s_sum[w], at_tile += s_sum_tile[w];
+    for (int b = 2 * b0; b < 2 * (b0 + per) && b < bins; ++b) {
+        const int sum = s_start[b];
+        s_to[b] = at + counts[(size_t)b * tiles + blockIdx.x] - at_tile;
+        s_start[b] = (unsigned short)at_tile;
+        at += total[b];
+        at_tile += sum;
     }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kSortItems; ++k) {
         const int i = first + k * 32;
-        if (i >= n || i < 0) continue;
-        const unsigned digit = (key[k] >> shift) & (bins - 1);
-        const int to = s_base[digit] + my[digit] + rank[k];
-        keys_out[to] = key[k];
-        pos_out[to] = FIRST ? i : pos[i];
+        const unsigned digit = (word[k].x >> shift) & (bins - 1);
+        if (i < n && i >= 0) s_word[s_start[digit] + my[digit] + rank[k]] = word[k];
+    }
+    __syncthreads();
+    const int count = min(n - base, kTile);
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k) {
+        const int i = k * kSortThreads + threadIdx.x;
+        if (i >= count) break;
+        const uint2 w = s_word[i];
+        words_out[s_to[(w.x >> shift) & (bins - 1)] + i] = w;
     }
 }
 
@@ -195,12 +224,10 @@ __global__ void __launch_bounds__(kSortThreads) k_digit_scatter(const void* __re
 constexpr int kFewIds = 4096, kFewThreads = 1024;
 
 __global__ void __launch_bounds__(kFewThreads) k_sort_few(const void* __restrict__ ids, int ids64, long long rows, long long padding, int n,
-                                                          int size, unsigned* __restrict__ keys_out, int* __restrict__ pos_out,
-                                                          int2* __restrict__ segment) {
+                                                          int size, uint2* __restrict__ words_out, int2* __restrict__ segment, int* __restrict__ popular) {
     const int threads = blockDim.x;   // up to half of `size`, the power of two from 64 on that holds n
     if (blockIdx.x) {
-        for (long long v = (long long)(blockIdx.x - 1) * threads + threadIdx.x; v < rows; v += (long long)(gridDim.x - 1) * threads)
-            segment[v] = make_int2(0, 0);
+        empty_segments(segment, popular, rows, (long long)(blockIdx.x - 1) * threads + threadIdx.x, (long long)(gridDim.x - 1) * threads);
         return;
     }
     __shared__ unsigned long long s_word[kFewIds];
@@ -224,8 +251,7 @@ __global__ void __launch_bounds__(kFewThreads) k_sort_few(const void* __restrict
     }
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += threads) {
-        keys_out[i] = (unsigned)(s_word[i] >> 32);
-        pos_out[i] = (int)(unsigned)s_word[i];
+        words_out[i] = make_uint2((unsigned)(s_word[i] >> 32), (unsigned)s_word[i]);
     }
 }
 
@@ -234,7 +260,8 @@ __global__ void __launch_bounds__(kFewThreads) k_sort_few(const void* __restrict
 // ----------------------------------------------------------------------------------------------
 // The sorted positions are cut into blocks of 64 and spans of several blocks.  A block whose positions all name one row is summed
 // ahead (a span of one row as a whole), all of them in parallel, so that a row with a hundred thousand positions is not one
-// group's work; k_sums then walks a row's segment and takes a span's or a block's sum where the segment holds all of it.
+// group's work.  Rows with such blocks are noted in a list (popular[0] of them, in any order) and get a CTA each, the
+// first ones of k_sums: as part of their neighbours' work they were its last 60 us where others were done.
 constexpr int kBlock = 64, kSpanWarps = kThreads / 32;
 
 template <class T, int VEC>
@@ -263,20 +290,21 @@ __device__ __forceinline__ void sum_block(float (&acc)[VEC], const T* __restrict
 
 // One CTA a span: notes where segments begin and end, and sums its uniform blocks.
 template <class T, int VEC, int G>
-__global__ void __launch_bounds__(kThreads) k_block_sums(const T* __restrict__ g, long long stride, const unsigned* __restrict__ keys,
-                                                         const int* __restrict__ pos, int n, unsigned rows, int F, int span,
+__global__ void __launch_bounds__(kThreads) k_block_sums(const T* __restrict__ g, long long stride, const uint2* __restrict__ words, int n, unsigned rows, int F, int span,
                                                          int2* __restrict__ segment, float* __restrict__ block_sum,
-                                                         float* __restrict__ span_sum) {
+                                                         float* __restrict__ span_sum, int* __restrict__ popular) {
     wait_for_kernel_before();
     const int p0 = blockIdx.x * span, p1 = min(n - p0, span) + p0;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, pieces = F / VEC;
-    const bool whole = p1 - p0 == span && keys[p0] == keys[p1 - 1] && keys[p0] < rows;
+    const bool whole = p1 - p0 == span && words[p0].x == words[p1 - 1].x && words[p0].x < rows;
     for (int b = p0 + warp * kBlock; b < p1; b += kSpanWarps * kBlock) {
         const int i0 = b + lane, i1 = i0 + 32;
-        const unsigned none = ~0u, k0 = i0 < n ? keys[i0] : none, k1 = i1 < n ? keys[i1] : none;
+        const unsigned none = ~0u;
+        const uint2 w0 = i0 < n ? words[i0] : make_uint2(none, 0), w1 = i1 < n ? words[i1] : make_uint2(none, 0);
+        const unsigned k0 = w0.x, k1 = w1.x;
         unsigned edge = none;   // the keys around the block
-        if (lane == 0 && b > 0) edge = keys[b - 1];
-        if (lane == 31 && b + kBlock < n) edge = keys[b + kBlock];
+        if (lane == 0 && b > 0) edge = words[b - 1].x;
+        if (lane == 31 && b + kBlock < n) edge = words[b + kBlock].x;
         const unsigned k0_up = __shfl_up_sync(none, k0, 1), k1_up = __shfl_up_sync(none, k1, 1), k0_down = __shfl_down_sync(none, k0, 1),
                        k1_down = __shfl_down_sync(none, k1, 1), k0_last = __shfl_sync(none, k0, 31), k1_first = __shfl_sync(none, k1, 0);
         auto note = [&](int i, unsigned k, unsigned before, unsigned after) {
@@ -287,10 +315,11 @@ __global__ void __launch_bounds__(kThreads) k_block_sums(const T* __restrict__ g
         };
         note(i0, k0, lane ? k0_up : edge, lane < 31 ? k0_down : k1_first);
         note(i1, k1, lane ? k1_up : k0_last, lane < 31 ? k1_down : edge);
-        if (whole) continue;
         const unsigned key = __shfl_sync(none, k0, 0);
         if (!__all_sync(none, k0 == key && k1 == key) || key >= rows) continue;   // (the end of the list is not: none)
-        const int pa = pos[i0], pb = pos[i1];
+        if (lane == 0 && (b == 0 || words[b - kBlock].x != key)) popular[1 + atomicAdd(popular, 1)] = (int)key;   // its first block
+        if (whole) continue;
+        const int pa = (int)w0.y, pb = (int)w1.y;
         for (int c0 = 0; c0 < pieces; c0 += G) {
             const int c = c0 + lane % G;
             float acc[VEC];
@@ -309,7 +338,7 @@ __global__ void __launch_bounds__(kThreads) k_block_sums(const T* __restrict__ g
         for (int k = 0; k < VEC; ++k) sum[k] = 0.f;
         for (int b = p0 + warp * kBlock; b < p1; b += kSpanWarps * kBlock) {
             float acc[VEC];
-            sum_block<T, VEC, G>(acc, g, stride, pos[b + lane], pos[b + 32 + lane], c, pieces);
+            sum_block<T, VEC, G>(acc, g, stride, (int)words[b + lane].y, (int)words[b + 32 + lane].y, c, pieces);
 #pragma unroll
             for (int k = 0; k < VEC; ++k) sum[k] += acc[k];
         }
@@ -326,10 +355,12 @@ __global__ void __launch_bounds__(kThreads) k_block_sums(const T* __restrict__ g
     }
 }
 
-// A group of G lanes writes kSumRows neighbouring rows, G pieces of each.  Their positions are neighbours too: where no row has a block's
-// worth of them, the group streams through them, kSumBatch at a time, and writes a row when the key changes; otherwise it goes
-// row by row and takes the blocks' and spans' sums.
-constexpr int kSumRows = 8, kSumBatch = 8, kPartBatch = 4;
+// A group of G lanes writes kSumRows neighbouring rows, G pieces of each.  Their positions are neighbours too: where none of the rows is
+// popular, the group streams through them, kSumBatch at a time, and writes a row when the key changes; otherwise it goes row by row.
+constexpr int kSumThreads = 128, kSumRows = 8, kSumBatch = 8;
+
+__device__ __forceinline__ int block_up(int p) { return (p + kBlock - 1) & ~(kBlock - 1); }
+__device__ __forceinline__ bool is_popular(int2 s) { return block_up(s.x) + kBlock <= s.y; }   // holds a block
 
 template <class TO, int VEC>
 __device__ __forceinline__ void write_sum(TO* __restrict__ o, const float (&acc)[VEC], float scale, int accumulate) {
@@ -340,108 +371,130 @@ __device__ __forceinline__ void write_sum(TO* __restrict__ o, const float (&acc)
     *(Piece<TO, VEC>*)o = q;
 }
 
+// What k_sums gets.
+template <class TI, class TO>
+struct SumArgs {
+    const TI* g;
+    long long stride;
+    const uint2* words;
+    int n;
+    long long rows;
+    int F, slabs, span;
+    const int2* segment;
+    const float *block_sum, *span_sum;
+    const int* popular;
+    int popular_ctas;
+    float scale;
+    TO* out;
+    long long out_stride;
+    int accumulate;
+};
+
+// A popular row by a CTA: its groups of lanes take the positions outside whole blocks, the blocks outside whole spans and the
+// spans in turn, and their sums are added in order.
 template <class TI, class TO, int VEC, int G>
-__global__ void __launch_bounds__(kThreads) k_sums(const TI* __restrict__ g, long long stride, const unsigned* __restrict__ keys,
-                                                   const int* __restrict__ pos, int n, long long rows, int F, int slabs, int span,
-                                                   const int2* __restrict__ segment, const float* __restrict__ block_sum,
-                                                   const float* __restrict__ span_sum, float scale, TO* __restrict__ out,
-                                                   long long out_stride, int accumulate) {
+__device__ __forceinline__ void sum_popular(const SumArgs<TI, TO>& a, long long v, float (*s_part)[G * VEC]) {
+    constexpr int GROUPS = kSumThreads / G;
+    const int group = threadIdx.x / G, lane = threadIdx.x % G, pieces = a.F / VEC;
+    const int2 s = a.segment[v];
+    const int b0 = block_up(s.x), b1 = s.y & ~(kBlock - 1);                               // whole blocks
+    const int t0 = (int)min(((long long)b0 + a.span - 1) / a.span * a.span, (long long)b1), t1 = max(b1 / a.span * a.span, t0);   // whole spans
+    const int head = b0 - s.x, singles = head + s.y - b1;
+    const int before = (t0 - b0) / kBlock, spans = (t1 - t0) / a.span, parts = before + spans + (b1 - t1) / kBlock;
+    for (int c0 = 0; c0 < pieces; c0 += G) {
+        const int c = c0 + lane;
+        float acc[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+        if (c < pieces) {
+#pragma unroll 4
+            for (int i = group; i < singles; i += GROUPS)
+                add_row<TI, VEC>(acc, a.g + (size_t)a.words[i < head ? s.x + i : b1 + i - head].y * a.stride, c);
+#pragma unroll 4
+            for (int i = group; i < parts; i += GROUPS) {
+                const float* from = i < before           ? a.block_sum + (size_t)(b0 / kBlock + i) * a.F
+                                    : i < before + spans ? a.span_sum + (size_t)(t0 / a.span + i - before) * a.F
+                                                         : a.block_sum + (size_t)(t1 / kBlock + i - before - spans) * a.F;
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) acc[k] += from[c * VEC + k];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) s_part[group][lane * VEC + k] = acc[k];
+        __syncthreads();
+        if (group == 0 && c < pieces) {
+            for (int w = 1; w < GROUPS; ++w)
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) acc[k] += s_part[w][lane * VEC + k];
+            write_sum<TO, VEC>(a.out + v * a.out_stride + (size_t)c * VEC, acc, a.scale, a.accumulate);
+        }
+        __syncthreads();
+    }
+}
+
+template <class TI, class TO, int VEC, int G>
+__global__ void __launch_bounds__(kSumThreads) k_sums(const SumArgs<TI, TO> a) {
+    __shared__ float s_part[kSumThreads / G][G * VEC];
     wait_for_kernel_before();
-    const long long item = ((long long)blockIdx.x * kThreads + threadIdx.x) / G, set = slabs == 1 ? item : item / slabs;
-    const long long v0 = set * kSumRows;
-    const int c = (slabs == 1 ? 0 : (int)(item - set * slabs) * G) + threadIdx.x % G;
-    if (v0 >= rows || c >= F / VEC) return;
-    g += (size_t)c * VEC;
-    out += v0 * out_stride + (size_t)c * VEC;
-    int begin = n, end_all = 0;
-    bool blocks = false;
+    if ((int)blockIdx.x < a.popular_ctas) {
+        for (int i = blockIdx.x; i < a.popular[0]; i += a.popular_ctas) sum_popular<TI, TO, VEC, G>(a, a.popular[1 + i], s_part);
+        return;
+    }
+    const long long item = ((long long)(blockIdx.x - a.popular_ctas) * kSumThreads + threadIdx.x) / G;
+    const long long set = a.slabs == 1 ? item : item / a.slabs, v0 = set * kSumRows;
+    const int c = (a.slabs == 1 ? 0 : (int)(item - set * a.slabs) * G) + threadIdx.x % G;
+    if (v0 >= a.rows || c >= a.F / VEC) return;
+    const TI* __restrict__ g = a.g + (size_t)c * VEC;
+    TO* __restrict__ out = a.out + v0 * a.out_stride + (size_t)c * VEC;
+    int begin = a.n, end_all = 0;
+    bool popular = false;
     {
         int2 s[kSumRows];
 #pragma unroll
-        for (int u = 0; u < kSumRows; ++u) s[u] = n > 0 && v0 + u < rows ? segment[v0 + u] : make_int2(0, 0);
+        for (int u = 0; u < kSumRows; ++u) s[u] = a.n > 0 && v0 + u < a.rows ? a.segment[v0 + u] : make_int2(0, 0);
 #pragma unroll
         for (int u = 0; u < kSumRows; ++u) {
             if (s[u].x < s[u].y) {
                 begin = min(begin, s[u].x);
                 end_all = max(end_all, s[u].y);
-                blocks |= s[u].y - s[u].x >= kBlock;
-            } else if (!accumulate && v0 + u < rows) {
-                *(Piece<TO, VEC>*)(out + u * out_stride) = Piece<TO, VEC>{};
+                popular |= is_popular(s[u]);
+            } else if (!a.accumulate && v0 + u < a.rows) {
+                *(Piece<TO, VEC>*)(out + u * a.out_stride) = Piece<TO, VEC>{};
             }
         }
     }
-    if (!blocks) {
+    // the rows of positions [p, end), written when the key changes
+    auto stream = [&](int p, int end) {
         float acc[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
-        for (int p = begin; p < end_all; p += kSumBatch) {
-            int at[kSumBatch];
-            unsigned key[kSumBatch + 1];
+        for (; p < end; p += kSumBatch) {
+            uint2 w[kSumBatch + 1];
 #pragma unroll
-            for (int k = 0; k < kSumBatch; ++k) at[k] = p + k < end_all ? pos[p + k] : -1;
-#pragma unroll
-            for (int k = 0; k <= kSumBatch; ++k) key[k] = p + k < end_all ? keys[p + k] : ~0u;
+            for (int k = 0; k <= kSumBatch; ++k) w[k] = p + k < end ? a.words[p + k] : make_uint2(~0u, 0);
             Piece<TI, VEC> row[kSumBatch];
 #pragma unroll
             for (int k = 0; k < kSumBatch; ++k)
-                if (at[k] >= 0) row[k] = *(const Piece<TI, VEC>*)(g + (size_t)at[k] * stride);
+                if (p + k < end) row[k] = *(const Piece<TI, VEC>*)(g + (size_t)w[k].y * a.stride);
 #pragma unroll
             for (int k = 0; k < kSumBatch; ++k) {
-                if (at[k] < 0) break;
+                if (p + k >= end) break;
                 add_piece(acc, row[k]);
-                if (key[k] == key[k + 1]) continue;
-                write_sum<TO, VEC>(out + (long long)(key[k] - (unsigned)v0) * out_stride, acc, scale, accumulate);
+                if (w[k].x == w[k + 1].x) continue;
+                write_sum<TO, VEC>(out + (long long)(w[k].x - (unsigned)v0) * a.out_stride, acc, a.scale, a.accumulate);
 #pragma unroll
                 for (int q = 0; q < VEC; ++q) acc[q] = 0.f;
             }
         }
-        return;
-    }
-#pragma unroll 1
-    for (int u = 0; u < kSumRows; ++u) {
-        if (v0 + u >= rows) break;
-        const int2 s = segment[v0 + u];
-        int p = s.x;
-        const int end = s.y;
-        if (p == end) continue;
-        float acc[VEC];
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
-        while (p < end) {
-            // whole blocks and spans from their sums, single positions otherwise
-            if ((p & (kBlock - 1)) == 0 && p + kBlock <= end) {
-                const bool spans = p % span == 0 && p + span <= end;
-                const int step = spans ? span : kBlock;
-                const float* from = (spans ? span_sum + (size_t)(p / span) * F : block_sum + (size_t)(p / kBlock) * F) + c * VEC;
-                // blocks up to the next span (which is taken as one) or the segment's end
-                const int stop = spans ? end : min(end, p - p % span + span), count = min((stop - p) / step, kPartBatch);
-                Piece<float, VEC> part[kPartBatch];
-#pragma unroll
-                for (int k = 0; k < kPartBatch; ++k)
-#pragma unroll
-                    for (int q = 0; q < VEC; ++q) part[k].v[q] = k < count ? from[(size_t)k * F + q] : 0.f;
-#pragma unroll
-                for (int k = 0; k < kPartBatch; ++k)
-#pragma unroll
-                    for (int q = 0; q < VEC; ++q) acc[q] += part[k].v[q];
-                p += count * step;
-            } else {
-                const int stop = min(end, (p & ~(kBlock - 1)) + kBlock);
-                Piece<TI, VEC> row[kSumBatch];
-                int at[kSumBatch];
-#pragma unroll
-                for (int k = 0; k < kSumBatch; ++k) at[k] = p + k < stop ? pos[p + k] : -1;
-#pragma unroll
-                for (int k = 0; k < kSumBatch; ++k) {
-                    row[k] = Piece<TI, VEC>{};
-                    if (at[k] >= 0) row[k] = *(const Piece<TI, VEC>*)(g + (size_t)at[k] * stride);
-                }
-#pragma unroll
-                for (int k = 0; k < kSumBatch; ++k) add_piece(acc, row[k]);
-                p = min(p + kSumBatch, stop);
-            }
+    };
+    const int runs = popular ? kSumRows : 1;
+    for (int u = 0; u < runs; ++u) {
+        int2 s = make_int2(begin, end_all);
+        if (popular) {
+            s = v0 + u < a.rows ? a.segment[v0 + u] : make_int2(0, 0);
+            if (is_popular(s)) continue;
         }
-        write_sum<TO, VEC>(out + u * out_stride, acc, scale, accumulate);
+        stream(s.x, s.y);
     }
 }
 
@@ -481,7 +534,7 @@ constexpr int kMaxFeatures = 1 << 20;
 
 struct GradPlan {
     int digits = 0, digit_bits = 0, tiles = 0, span = 0, spans = 0;
-    size_t keys[2] = {}, pos[2] = {}, counts = 0, total = 0, segment = 0, block_sum = 0, span_sum = 0, bytes = 0;
+    size_t words[2] = {}, counts = 0, total = 0, segment = 0, block_sum = 0, span_sum = 0, popular = 0, bytes = 0;
 };
 
 GradPlan grad_plan(long long n, long long rows, int F) {
@@ -501,15 +554,13 @@ GradPlan grad_plan(long long n, long long rows, int F) {
         at += (bytes + 255) & ~(size_t)255;
         return here;
     };
-    for (int k = 0; k < 2; ++k) {
-        p.keys[k] = take((size_t)n * 4);
-        p.pos[k] = take((size_t)n * 4);
-    }
+    for (int k = 0; k < 2; ++k) p.words[k] = take((size_t)n * 8);
     p.counts = take(((size_t)p.tiles << p.digit_bits) * 4);
     p.total = take((size_t)4 << p.digit_bits);
-    p.segment = take((size_t)rows * 8);
+    p.segment = take((size_t)(rows + 1) * 8);
     p.block_sum = take((size_t)(n / kBlock) * F * 4);
     p.span_sum = take((size_t)p.spans * F * 4);
+    p.popular = take((size_t)(n / kBlock + 1) * 4);
     p.bytes = at;
     return p;
 }
@@ -526,19 +577,18 @@ template <bool FIRST>
 int sort_pass(const void* ids, int ids64, long long rows, long long padding, unsigned char* ws, const GradPlan& p, int n, int pass,
               cudaStream_t st) {
     const int from = (pass + 1) & 1, to = pass & 1, shift = pass * p.digit_bits, bins = 1 << p.digit_bits;
-    const unsigned* keys = (const unsigned*)(ws + p.keys[from]);
-    const int* pos = (const int*)(ws + p.pos[from]);
+    const uint2* words = (const uint2*)(ws + p.words[from]);
     int *counts = (int*)(ws + p.counts), *total = (int*)(ws + p.total);
-    int rc = launch_behind(k_digit_counts<FIRST>, dim3(p.tiles), kSortThreads, (size_t)bins * 4, st, !FIRST, ids, ids64, rows, padding, keys, n, shift,
-                    p.digit_bits, counts, (int2*)(ws + p.segment));
+    int rc = launch_behind(k_digit_counts<FIRST>, dim3(p.tiles), kSortThreads, (size_t)bins * 4, st, !FIRST, ids, ids64, rows, padding, words, n, shift,
+                    p.digit_bits, counts, (int2*)(ws + p.segment), (int*)(ws + p.popular));
     if (rc) return rc;
     rc = launch_behind(k_digit_prefix, dim3(ceil_div(bins, 8)), 256, 0, st, true, counts, p.tiles, bins, total);
     if (rc) return rc;
-    const size_t smem = (size_t)bins * (4 + 2 * kSortWarps);
-    rc = allow_smem(k_digit_scatter<FIRST>, (1 << kMaxDigit) * (4 + 2 * kSortWarps), false, g_scatter_done[FIRST]);
+    auto smem = [](int bins) { return kTile * 8 + bins * (6 + 2 * kSortWarps); };
+    rc = allow_smem(k_digit_scatter<FIRST>, smem(1 << kMaxDigit), false, g_scatter_done[FIRST]);
     if (rc) return rc;
-    return launch_behind(k_digit_scatter<FIRST>, dim3(p.tiles), kSortThreads, smem, st, true, ids, ids64, rows, padding, keys, pos, n, shift, p.digit_bits,
-                  (const int*)counts, (const int*)total, (unsigned*)(ws + p.keys[to]), (int*)(ws + p.pos[to]));
+    return launch_behind(k_digit_scatter<FIRST>, dim3(p.tiles), kSortThreads, (size_t)smem(bins), st, true, ids, ids64, rows, padding, words, n, shift, p.digit_bits,
+                  (const int*)counts, (const int*)total, (uint2*)(ws + p.words[to]));
 }
 
 }  // namespace
@@ -607,8 +657,8 @@ extern "C" int trs_embedding_grad(const void* grad, int grad_type, long long gra
             while (size < n) size *= 2;
             const int threads = size / 2 < kFewThreads ? size / 2 : kFewThreads;
             const long long zero = ceil_div64(rows, 4 * threads);
-            rc = launch(k_sort_few, dim3(1 + (unsigned)(zero < 2 * 148 ? zero : 2 * 148)), threads, 0, st, ids, ids64, rows, padding_id, (int)n, size, (unsigned*)(ws + p.keys[0]),
-                        (int*)(ws + p.pos[0]), (int2*)(ws + p.segment));
+            rc = launch(k_sort_few, dim3(1 + (unsigned)(zero < 2 * 148 ? zero : 2 * 148)), threads, 0, st, ids, ids64, rows, padding_id, (int)n, size,
+                        (uint2*)(ws + p.words[0]), (int2*)(ws + p.segment), (int*)(ws + p.popular));
             if (rc) return rc;
         } else for (int pass = 0; pass < p.digits; ++pass) {
             rc = pass == 0 ? sort_pass<true>(ids, ids64, rows, padding_id, ws, p, (int)n, pass, st)
@@ -617,10 +667,10 @@ extern "C" int trs_embedding_grad(const void* grad, int grad_type, long long gra
         }
     }
     const int last = (p.digits + 1) & 1;
-    const unsigned* keys = (const unsigned*)(ws + p.keys[last]);
-    const int* pos = (const int*)(ws + p.pos[last]);
+    const uint2* words = (const uint2*)(ws + p.words[last]);
     int2* segment = (int2*)(ws + p.segment);
     float *block_sum = (float*)(ws + p.block_sum), *span_sum = (float*)(ws + p.span_sum);
+    int* popular = (int*)(ws + p.popular);
     const int vec = elements_per_piece(F, grad, grad_type, grad_stride, out, out_type, out_stride), pieces = F / vec;
     return with_type(grad_type, [&](auto ti) {
         using TI = decltype(ti);
@@ -632,8 +682,8 @@ extern "C" int trs_embedding_grad(const void* grad, int grad_type, long long gra
                 return with_group(pieces, [&](auto gr) {
                     constexpr int G = decltype(gr)::value;
                     if (n) {
-                        const int e = launch_behind(k_block_sums<TI, VEC, G>, dim3(p.spans), kThreads, 0, st, true, (const TI*)grad, grad_stride, keys, pos,
-                                                    (int)n, (unsigned)rows, F, p.span, segment, block_sum, span_sum);
+                        const int e = launch_behind(k_block_sums<TI, VEC, G>, dim3(p.spans), kThreads, 0, st, true, (const TI*)grad, grad_stride, words,
+                                                    (int)n, (unsigned)rows, F, p.span, segment, block_sum, span_sum, popular);
                         if (e) return e;
                     }
                     return with_type(out_type, [&](auto to) {
@@ -643,10 +693,12 @@ extern "C" int trs_embedding_grad(const void* grad, int grad_type, long long gra
                         } else {
                             const int slabs = ceil_div(pieces, G);
                             const long long threads = ceil_div64(rows, kSumRows) * slabs * G;
-                            if (ceil_div64(threads, kThreads) > 0x7fffffffll) return (int)TRS_E_LIMIT;
-                            return launch_behind(k_sums<TI, TO, VEC, G>, dim3((unsigned)ceil_div64(threads, kThreads)), kThreads, 0, st, n > 0,
-                                                 (const TI*)grad, grad_stride, keys, pos, (int)n, rows, F, slabs, p.span, (const int2*)segment,
-                                                 (const float*)block_sum, (const float*)span_sum, scale, (TO*)out, out_stride, accumulate);
+                            if (ceil_div64(threads, kSumThreads) > 0x7fff0000ll) return (int)TRS_E_LIMIT;
+                            const int popular_ctas = (int)(n / kBlock < 2 * 148 ? n / kBlock : 2 * 148);
+                            const SumArgs<TI, TO> args{(const TI*)grad, grad_stride, words, (int)n, rows, F, slabs, p.span, segment, block_sum, span_sum,
+                                                       popular, popular_ctas, scale, (TO*)out, out_stride, accumulate};
+                            return launch_behind(k_sums<TI, TO, VEC, G>, dim3((unsigned)(popular_ctas + ceil_div64(threads, kSumThreads))),
+                                                 kSumThreads, 0, st, n > 0, args);
                         }
                     });
                 });
