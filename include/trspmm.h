@@ -372,8 +372,8 @@ int trs_sddmm_plan_destroy(trs_sddmm_plan* plan);
  * table: [rows, F], out: [n, F], of TRS_TYPE_* each, rows `*_stride` >= F elements apart.  ids: [n] of 32 or
  * (ids64 != 0) 64 bits.  An id equal to padding_id gives a row of zeros (TRS_NO_PADDING: no such id); an id outside
  * [0, rows) gives a row of NaN, and nothing outside the table is read.  n = 0 does nothing.  `out` may not
- * overlap the table.  Asynchronous on `stream`; allocates nothing.  Up to 2^31 - 65536 ids, 2^31 - 2 rows, 2^20 features
- * (TRS_E_LIMIT beyond). */
+ * overlap the table.  Asynchronous on `stream`; allocates nothing.  Up to 2^31 - 65536 ids, 2^31 - 2 rows, 2^20 features,
+ * strides below 2^31 (TRS_E_LIMIT beyond). */
 #define TRS_NO_PADDING INT64_MIN
 int trs_embedding(const void* table, int table_type, long long rows, long long table_stride, const void* ids, int ids64,
                   long long n, int F, float scale, long long padding_id, void* out, int out_type, long long out_stride,

@@ -20,37 +20,51 @@ __device__ __forceinline__ long long load_id(const void* __restrict__ ids, int i
 // ----------------------------------------------------------------------------------------------
 // Lookup
 // ----------------------------------------------------------------------------------------------
-// A group of G lanes copies kLookupRows rows at a time, piece by piece, so that a thread has as many loads in flight.
-constexpr int kThreads = 256, kLookupRows = 4;
+// A group of G lanes copies ROWS rows at a time, PER pieces a lane, so that a thread has ROWS x PER loads in flight, with no branch around
+// them.  COPY: the result has the table's type and the factor is 1, so the bits are moved as they are.  Bound by DRAM: 2^20
+// popular rows of 128 fp16 features 66 us, 5.1 TB/s of the rows that are named, the ids and the result.
+constexpr int kThreads = 256, kLookupThreads = 128;
 
-template <class TI, class TO, int VEC, int G>
-__global__ void __launch_bounds__(kThreads) k_lookup(const TI* __restrict__ table, long long rows, long long stride,
-                                                     const void* __restrict__ ids, int ids64, long long n, int pieces, float scale,
-                                                     long long padding, TO* __restrict__ out, long long out_stride) {
-    const long long group = ((long long)blockIdx.x * kThreads + threadIdx.x) / G;
-    const int lane = threadIdx.x % G;
-    const long long i0 = group * kLookupRows;
+template <class TI, class TO, int VEC, int G, int ROWS, int PER, bool COPY>
+__global__ void __launch_bounds__(kLookupThreads) k_lookup(const TI* __restrict__ table, unsigned rows, unsigned stride,
+                                                           const void* __restrict__ ids, int ids64, unsigned n, int pieces, float scale,
+                                                           long long padding, TO* __restrict__ out, unsigned out_stride) {
+    const unsigned group = (blockIdx.x * kLookupThreads + threadIdx.x) / G, i0 = group * ROWS;
+    int c = threadIdx.x % G;
     if (i0 >= n) return;
-    const TI* from[kLookupRows];
-    float mul[kLookupRows];
+    const TI* from[ROWS];
+    bool none[ROWS];   // no row to read: the result is zeros times `mul`
+    float mul[ROWS];
 #pragma unroll
-    for (int u = 0; u < kLookupRows; ++u) {
-        const long long id = i0 + u < n ? load_id(ids, ids64, i0 + u) : -1;
-        const bool pad = id == padding && padding != TRS_NO_PADDING, bad = (unsigned long long)id >= (unsigned long long)rows;
-        from[u] = pad || bad ? nullptr : table + id * stride + lane * VEC;
-        mul[u] = pad ? 0.f : bad ? __int_as_float(0x7fffffff) : scale;   // what zeros are multiplied by where there is no row
+    for (int u = 0; u < ROWS; ++u) {
+        const long long id = load_id(ids, ids64, min(i0 + u, n - 1));
+        const bool pad = id == padding && padding != TRS_NO_PADDING;
+        none[u] = pad || (unsigned long long)id >= rows;
+        mul[u] = pad ? 0.f : none[u] ? __int_as_float(0x7fffffff) : scale;
+        from[u] = table + (size_t)(none[u] ? 0u : (unsigned)id) * stride;   // (row 0 in its place: no branch around the load)
     }
-    TO* to = out + i0 * out_stride + lane * VEC;
-    for (int c = lane; c < pieces; c += G) {
-        Piece<TI, VEC> p[kLookupRows];
+    TO* to = out + (size_t)i0 * out_stride;
+    for (; c < pieces; c += PER * G) {
+        Piece<TI, VEC> p[ROWS][PER];
 #pragma unroll
-        for (int u = 0; u < kLookupRows; ++u) {
-            p[u] = Piece<TI, VEC>{};
-            if (from[u]) p[u] = *(const Piece<TI, VEC>*)(from[u] + (c - lane) * VEC);
+        for (int u = 0; u < ROWS; ++u)
+#pragma unroll
+            for (int i = 0; i < PER; ++i) p[u][i] = *(const Piece<TI, VEC>*)(from[u] + min(c + i * G, pieces - 1) * VEC);
+#pragma unroll
+        for (int u = 0; u < ROWS; ++u) {
+            if (i0 + u >= n) break;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                if (i && c + i * G >= pieces) break;
+                if (none[u]) {
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) p[u][i].v[k] = from_float<TI>(COPY ? mul[u] : 0.f);
+                }
+                Piece<TO, VEC>* o = (Piece<TO, VEC>*)(to + (size_t)u * out_stride + (c + i * G) * VEC);
+                if constexpr (COPY) *o = *(const Piece<TO, VEC>*)&p[u][i];
+                else *o = scaled<TO>(p[u][i], mul[u]);
+            }
         }
-#pragma unroll
-        for (int u = 0; u < kLookupRows; ++u)
-            if (i0 + u < n) *(Piece<TO, VEC>*)(to + u * out_stride + (c - lane) * VEC) = scaled<TO>(p[u], mul[u]);
     }
 }
 
@@ -277,10 +291,17 @@ __device__ __forceinline__ void sum_block(float (&acc)[VEC], const T* __restrict
     const int group = threadIdx.x % 32 / G;
 #pragma unroll
     for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < kBlock / GROUPS; ++i) {
-        const int j = i * GROUPS + group, p = __shfl_sync(0xffffffffu, i < kBlock / GROUPS / 2 ? pa : pb, j % 32);
-        if (c < pieces) add_row<T, VEC>(acc, g + (size_t)p * stride, c);
+    constexpr int BATCH = 8;
+    for (int i0 = 0; i0 < kBlock / GROUPS; i0 += BATCH) {
+        Piece<T, VEC> row[BATCH];
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            const int j = (i0 + k) * GROUPS + group, p = __shfl_sync(0xffffffffu, j < 32 ? pa : pb, j % 32);
+            row[k] = Piece<T, VEC>{};
+            if (c < pieces) row[k] = *(const Piece<T, VEC>*)(g + (size_t)p * stride + (size_t)c * VEC);
+        }
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) add_piece(acc, row[k]);
     }
 #pragma unroll
     for (int o = G; o < 32; o *= 2)
@@ -290,7 +311,7 @@ __device__ __forceinline__ void sum_block(float (&acc)[VEC], const T* __restrict
 
 // One CTA a span: notes where segments begin and end, and sums its uniform blocks.
 template <class T, int VEC, int G>
-__global__ void __launch_bounds__(kThreads) k_block_sums(const T* __restrict__ g, long long stride, const uint2* __restrict__ words, int n, unsigned rows, int F, int span,
+__global__ void __launch_bounds__(kThreads, 4) k_block_sums(const T* __restrict__ g, long long stride, const uint2* __restrict__ words, int n, unsigned rows, int F, int span,
                                                          int2* __restrict__ segment, float* __restrict__ block_sum,
                                                          float* __restrict__ span_sum, int* __restrict__ popular) {
     wait_for_kernel_before();
@@ -357,7 +378,7 @@ __global__ void __launch_bounds__(kThreads) k_block_sums(const T* __restrict__ g
 
 // A group of G lanes writes kSumRows neighbouring rows, G pieces of each.  Their positions are neighbours too: where none of the rows is
 // popular, the group streams through them, kSumBatch at a time, and writes a row when the key changes; otherwise it goes row by row.
-constexpr int kSumThreads = 128, kSumRows = 8, kSumBatch = 8;
+constexpr int kSumThreads = 128, kSumRows = 8, kSumBatch = 4;
 
 __device__ __forceinline__ int block_up(int p) { return (p + kBlock - 1) & ~(kBlock - 1); }
 __device__ __forceinline__ bool is_popular(int2 s) { return block_up(s.x) + kBlock <= s.y; }   // holds a block
@@ -451,10 +472,10 @@ __global__ void __launch_bounds__(kSumThreads) k_sums(const SumArgs<TI, TO> a) {
     {
         int2 s[kSumRows];
 #pragma unroll
-        for (int u = 0; u < kSumRows; ++u) s[u] = a.n > 0 && v0 + u < a.rows ? a.segment[v0 + u] : make_int2(0, 0);
+        for (int u = 0; u < kSumRows; ++u) s[u] = a.n > 0 ? a.segment[min(v0 + u, a.rows - 1)] : make_int2(0, 0);
 #pragma unroll
         for (int u = 0; u < kSumRows; ++u) {
-            if (s[u].x < s[u].y) {
+            if (s[u].x < s[u].y && v0 + u < a.rows) {
                 begin = min(begin, s[u].x);
                 end_all = max(end_all, s[u].y);
                 popular |= is_popular(s[u]);
@@ -529,7 +550,20 @@ int with_group(int pieces, Fn fn) {
     return fn(std::integral_constant<int, 32>());
 }
 
+// Lookup: lanes, rows and pieces in flight.  Few lanes a row spare instructions (what a lane spends on a row's id and address is as much
+// as it spends on three pieces): F = 47 of fp32 rows 27 us with 32 lanes x 4 rows, 17 us with 16 lanes x 2 rows x 3 pieces.
+template <class Fn>
+int with_lookup(int pieces, Fn fn) {
+    using std::integral_constant;
+    if (pieces <= 4) return fn(integral_constant<int, 4>(), integral_constant<int, 4>(), integral_constant<int, 1>());
+    if (pieces <= 8) return fn(integral_constant<int, 4>(), integral_constant<int, 4>(), integral_constant<int, 2>());
+    if (pieces <= 16) return fn(integral_constant<int, 8>(), integral_constant<int, 4>(), integral_constant<int, 2>());
+    if (pieces <= 32) return fn(integral_constant<int, 16>(), integral_constant<int, 2>(), integral_constant<int, 2>());
+    return fn(integral_constant<int, 16>(), integral_constant<int, 2>(), integral_constant<int, 3>());
+}
+
 constexpr long long kMaxIds = (1ll << 31) - (1 << 16), kMaxRows = (1ll << 31) - 2;
+constexpr long long kMaxStride = (1ll << 31) - 1;
 constexpr int kMaxFeatures = 1 << 20;
 
 struct GradPlan {
@@ -602,6 +636,7 @@ extern "C" int trs_embedding(const void* table, int table_type, long long rows, 
     const int rc = check_sizes(rows, n, F);
     if (rc) return rc;
     if (!type_known(table_type) || !type_known(out_type) || table_stride < F || out_stride < F) return TRS_E_ARG;
+    if (table_stride > kMaxStride || out_stride > kMaxStride) return TRS_E_LIMIT;
     if (n == 0) return TRS_OK;
     if (!table || !ids || !out) return TRS_E_ARG;
     const int vec = elements_per_piece(F, table, table_type, table_stride, out, out_type, out_stride), pieces = F / vec;
@@ -614,12 +649,17 @@ extern "C" int trs_embedding(const void* table, int table_type, long long rows, 
                 if constexpr (VEC * (sizeof(TI) > sizeof(TO) ? sizeof(TI) : sizeof(TO)) > 16) {
                     return (int)TRS_E_ARG;   // not reached: elements_per_piece
                 } else {
-                    return with_group(pieces, [&](auto gr) {
-                        constexpr int G = decltype(gr)::value;
-                        const long long groups = ceil_div64(n, kLookupRows);
-                        return launch(k_lookup<TI, TO, VEC, G>, dim3((unsigned)ceil_div64(groups * G, kThreads)), kThreads, 0,
-                                      (cudaStream_t)stream, (const TI*)table, rows, table_stride, ids, ids64, n, pieces, scale, padding_id,
-                                      (TO*)out, out_stride);
+                    return with_lookup(pieces, [&](auto gr, auto ro, auto pe) {
+                        constexpr int G = decltype(gr)::value, ROWS = decltype(ro)::value, PER = decltype(pe)::value;
+                        const dim3 grid((unsigned)ceil_div64(ceil_div64(n, ROWS) * G, kLookupThreads));
+                        auto run = [&](auto copy) {
+                            return launch(k_lookup<TI, TO, VEC, G, ROWS, PER, decltype(copy)::value>, grid, kLookupThreads, 0, (cudaStream_t)stream,
+                                          (const TI*)table, (unsigned)rows, (unsigned)table_stride, ids, ids64, (unsigned)n, pieces, scale, padding_id,
+                                          (TO*)out, (unsigned)out_stride);
+                        };
+                        if constexpr (std::is_same<TI, TO>::value)
+                            if (scale == 1.f) return run(std::true_type());
+                        return run(std::false_type());
                     });
                 }
             });

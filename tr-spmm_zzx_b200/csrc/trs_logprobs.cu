@@ -24,11 +24,18 @@ constexpr int kMaxTop = 32;
 
 typedef unsigned long long Key;   // (score, class): larger scores first, then lower classes; 0: none
 
-__device__ __forceinline__ Key key_of(float x, int j) {
-    const unsigned b = __float_as_uint(x + 0.f);   // -0 as 0
-    const unsigned up = b & 0x80000000u ? ~b : b | 0x80000000u;
-    return (Key)up << 32 | (unsigned)~j;
+// Unsigned numbers in the order of the scores; -0 as 0.
+__device__ __forceinline__ unsigned order_of(float x) {
+    const unsigned b = __float_as_uint(x + 0.f);
+    return b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
 }
+template <class T>
+__device__ __forceinline__ unsigned order_of_16(T x) {
+    unsigned b = *(const unsigned short*)&x;
+    if (b == 0x8000u) b = 0;
+    return b & 0x8000u ? b ^ 0xffffu : b | 0x8000u;
+}
+__device__ __forceinline__ Key key_of(float x, int j) { return (Key)order_of(x) << 32 | (unsigned)~j; }
 __device__ __forceinline__ float key_score(Key k) {
     const unsigned up = (unsigned)(k >> 32);
     return __uint_as_float(up & 0x80000000u ? up & 0x7fffffffu : ~up);
@@ -155,10 +162,11 @@ __device__ __forceinline__ void write_row(const Forward& a, long long r, const T
         a.logprobs[r] = lp;
     }
 }
-__device__ __forceinline__ void write_top(const Forward& a, long long r, int k, Key key, Sums s) {
-    const bool broken = !(s.m < INFINITY), has = key != 0 && !broken;
-    a.top_ids[r * a.top + k] = has ? key_class(key) : -1;
-    a.top_logprobs[r * a.top + k] = broken ? NAN : has ? (key_score(key) - s.m) * a.scale - logf(s.S) : -INFINITY;
+__device__ __forceinline__ void write_top(const Forward& a, long long r, int k, bool has, int id, float score, float m, float log_S) {
+    const bool broken = !(m < INFINITY);
+    has = has && !broken;
+    a.top_ids[r * a.top + k] = has ? id : -1;
+    a.top_logprobs[r * a.top + k] = broken ? NAN : has ? (score - m) * a.scale - log_S : -INFINITY;
 }
 
 __device__ __forceinline__ Key warp_max(Key k) {
@@ -528,14 +536,15 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_row(const Forward a
     } else if (a.top) {
         __syncthreads();
     }
-    for (int k = threadIdx.x; k < a.top; k += THREADS) write_top(a, r, k, s_best[k], s_all);
+    for (int k = threadIdx.x; k < a.top; k += THREADS)
+        write_top(a, r, k, s_best[k] != 0, key_class(s_best[k]), key_score(s_best[k]), s_all.m, logf(s_all.S));
 }
 
 // ----------------------------------------------------------------------------------------------
 // Short rows: a group of G lanes a row
 // ----------------------------------------------------------------------------------------------
 // The whole row is held in registers, PER pieces a lane (16 scores, or 32 for the longest), so the maximum comes first and the sums
-// after it.  An alternative is the group's maximum, then the lowest class that has it, taken out for the next one.
+// after it.
 constexpr int kShortThreads = 256;
 
 template <int G>
@@ -582,7 +591,46 @@ __global__ void __launch_bounds__(kShortThreads) k_short_rows(const Forward a) {
         }
     s = group_sum<G>(s);
     if (g == 0 && r == r0) write_row<T>(a, r, row.x, row.mask, s);
-    const bool broken = !(m < INFINITY);
+    if (!a.top) return;
+    const float log_S = logf(s.S);
+    // One word a score: as much of its order as fits above its class, so that a maximum of words is a maximum of scores with the lowest
+    // class first among equal ones.  16-bit scores fit; fp32 scores lose their lowest bits, and where two of the best (or the
+    // last and the next) agree in what is left, the warp takes the exact rounds below instead.
+    int bits = 16;
+    if constexpr (sizeof(T) == 4) bits = 32 - __clz(a.classes - 1 | 1);
+    const unsigned low = (1u << bits) - 1;
+    unsigned word[PER][VEC];
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+            const unsigned up = sizeof(T) == 4 ? order_of(v[i][k]) : order_of_16(from_float<T>(v[i][k])) << 16;
+            word[i][k] = v[i][k] > -INFINITY ? (up & ~low) | (low - (unsigned)(row.first(g + i * G) + k)) : 0u;
+        }
+    bool close = false;
+    unsigned last = ~0u, mine = 0;   // `mine`: the group's lanes take the found ones in turn, and write them together
+    for (int k = 0; k < a.top + (sizeof(T) == 4 ? 1 : 0); ++k) {
+        unsigned best = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) best = max(best, word[i][q] - last);   // (words below `last` wrap around to above the others)
+#pragma unroll
+        for (int o = G / 2; o; o /= 2) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+        const unsigned next = best + last;
+        const unsigned found = last == 0 || next >= last ? 0u : next;
+        if (sizeof(T) == 4 && k && found) close |= ((found ^ last) & ~low) == 0;
+        last = found;
+        if (k >= a.top) break;
+        if (k % G == g) mine = found;
+        if (k % G == G - 1 || k == a.top - 1) {
+            if (g <= k % G && r == r0) {
+                const int id = (int)(low - (mine & low));
+                write_top(a, r, k - k % G + g, mine != 0, id, mine ? as_float(row.x[id]) : 0.f, s.m, log_S);
+            }
+        }
+    }
+    if (sizeof(T) == 2 || !__any_sync(0xffffffffu, close)) return;
     for (int k = 0; k < a.top; ++k) {
         if (k) {
             m = -INFINITY;
@@ -606,7 +654,7 @@ __global__ void __launch_bounds__(kShortThreads) k_short_rows(const Forward a) {
 #pragma unroll
             for (int q = 0; q < VEC; ++q)
                 if (row.first(g + i * G) + q == at) v[i][q] = -INFINITY;
-        if (k % G == g && r == r0) write_top(a, r, k, broken || m == -INFINITY ? 0 : key_of(m, at), s);
+        if (k % G == g && r == r0) write_top(a, r, k, m > -INFINITY, at, m, s.m, log_S);
     }
 }
 
