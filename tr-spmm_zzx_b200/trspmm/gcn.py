@@ -14,6 +14,8 @@ import torch
 
 from . import shard
 from .builder import build_format
+from .embedding import embedding
+from .logprobs import ClassLogprobs, class_logprobs
 from .spmm import SpmmPlan
 
 
@@ -97,8 +99,29 @@ class ShardedGCN2:
             for w in dist.batch_isend_irecv(ops):
                 w.wait()
 
-    def forward(self, X: torch.Tensor, W1: torch.Tensor, W2: torch.Tensor, gather: str = "h1") -> torch.Tensor:
-        """X [N, F0] fp16 (replicated), W1 [F0, F1], W2 [F1, F2] fp16.  Returns this rank's rows of
+    def classify(self, X: torch.Tensor, W1: torch.Tensor, W2: torch.Tensor, labels: torch.Tensor | None = None, top: int = 1,
+                 gather: str = "h1", ids: torch.Tensor | None = None, ignore_id: int | None = None) -> ClassLogprobs:
+        """The forward pass, and what its F2 outputs say as scores over F2 classes: for this rank's rows the log probabilities
+        of their labels ([N], all nodes'), the entropies and the `top` best classes (class_logprobs)."""
+        out = self.forward(X, W1, W2, gather, ids)
+        own = None if labels is None else labels[self.r0:self.r1]
+        return class_logprobs(out, own, top=top, ignore_id=ignore_id)
+
+    def _first_product(self, X, W1, ids):
+        """X W1 of all nodes.  With ids the rows of X are looked up: behind the product where the table has fewer rows than the
+        graph has nodes (it is linear), before it otherwise."""
+        if ids is None:
+            return torch.matmul(X, W1)
+        if ids.shape != (self.n,):
+            raise ValueError(f"ids has shape {tuple(ids.shape)}, the graph {self.n} nodes")
+        if X.shape[0] <= self.n:
+            return embedding(torch.matmul(X, W1), ids)
+        return torch.matmul(embedding(X, ids), W1)
+
+    def forward(self, X: torch.Tensor, W1: torch.Tensor, W2: torch.Tensor, gather: str = "h1",
+                ids: torch.Tensor | None = None) -> torch.Tensor:
+        """X [N, F0] fp16 (replicated), W1 [F0, F1], W2 [F1, F2] fp16; with `ids` ([N], int64 or int32) X is a table of
+        feature rows, and node i has row ids[i].  Returns this rank's rows of
         the output, [r1 - r0, F2] fp16.  gather="h1" exchanges the hidden matrix (N x F1) with NCCL;
         gather="z2" multiplies the own rows by W2 first and exchanges N x F2 instead;
         gather="fused" lets the layer-1 SpMM store its rows into every rank's H1 itself
@@ -117,7 +140,7 @@ class ShardedGCN2:
                 marks.append((name, e))
 
         mark("start")
-        z1 = torch.matmul(X, W1)                                   # [N, F1], replicated compute
+        z1 = self._first_product(X, W1, ids)                       # [N, F1], replicated compute
         mark("gemm1")
         if gather == "h1":
             h1 = torch.empty((self.n, W1.shape[1]), dtype=torch.float16, device=X.device)
