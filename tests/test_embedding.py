@@ -60,7 +60,8 @@ def test_entries_refuse_bad_arguments_before_any_launch():
     for bad in (dict(table=None), dict(ids=None), dict(out=None), dict(rows=0), dict(n=-1), dict(F=0), dict(tt=3), dict(ot=-1),
                 dict(ts=7), dict(os=7)):
         assert look(**bad) == -1, bad
-    for big in (dict(rows=1 << 31), dict(n=1 << 31), dict(F=(1 << 20) + 1, ts=1 << 21, os=1 << 21)):
+    assert look(table=a + 2) == -1 and look(out=a + 1, ot=1) == -1 and look(ids=a + 4) == -1   # not on element boundaries
+    for big in (dict(rows=1 << 31), dict(n=1 << 31), dict(F=(1 << 20) + 1, ts=1 << 21, os=1 << 21), dict(ts=1 << 31), dict(os=1 << 31)):
         assert look(**big) == -10, big
     assert lib.trs_embedding_grad_workspace_bytes(10, 4, 8, None) == -1
     assert lib.trs_embedding_grad_workspace_bytes(10, 0, 8, ctypes.byref(sz)) == -1
@@ -72,6 +73,7 @@ def test_entries_refuse_bad_arguments_before_any_launch():
     for bad in (dict(g=None), dict(ids=None), dict(out=None), dict(rows=0), dict(n=-1), dict(F=0), dict(gt=3), dict(ot=3), dict(gs=7),
                 dict(os=7)):
         assert grad(**bad) == -1, bad
+    assert grad(g=a + 2) == -1 and grad(out=a + 1, ot=2) == -1 and grad(ids=a + 4) == -1
     assert grad(wb=100) == -7 and grad(ws=None, wb=1 << 30) == -7 and grad(ws=a + 8, wb=1 << 30) == -7
     assert grad(n=1 << 31) == -10
     assert grad(n=0, acc=1) == 0

@@ -160,7 +160,7 @@ def test_entries_refuse_bad_arguments_before_any_launch():
     assert fwd(n=0) == 0
     for bad in (dict(x=None), dict(x=a + 2), dict(ty=3), dict(ty=-1), dict(n=-1), dict(C=0), dict(st=3), dict(t=None), dict(scale=0.0),
                 dict(scale=-1.0), dict(scale=float("inf")), dict(scale=float("nan")), dict(top=-1), dict(top=1), dict(top=1, tl=a),
-                dict(mask=a, ms=3), dict(stats=a + 4), dict(ty=1, x=a + 1)):
+                dict(mask=a, ms=3), dict(stats=a + 4), dict(ty=1, x=a + 1), dict(t=a + 4), dict(lp=a + 2), dict(scale=3e38)):
         assert fwd(**bad) == -1, bad
     for big in (dict(n=1 << 31), dict(C=(1 << 30) + 1, st=1 << 31), dict(top=33, tl=a, ti=a)):
         assert fwd(**big) == -10, big
@@ -405,3 +405,24 @@ def test_streams_graphs_and_repeats(n, C):
     want = both()
     graph.replay()
     assert all(torch.equal(a, b) for a, b in zip(held, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C", [6, 47, 600, 5000, 66000])
+def test_rows_without_a_distribution_are_nan_wherever_they_lie(C):
+    """A NaN beside scores of -inf: the gradient is NaN in every place that is not masked, whichever alignment the row has."""
+    from trspmm import class_logprobs, class_logprobs_grad
+    for offset in (0, 1, 3):
+        x = _scores(5, C, F16, width=C + 8, offset=offset)
+        x[:, 1::2] = NEG
+        x[:, C - 2] = float("nan")
+        r = class_logprobs(x)
+        assert bool(torch.isnan(r.entropy).all())
+        keep = torch.arange(C, device="cuda") % 4 != 3
+        for mask in (None, keep):
+            d = class_logprobs_grad(x, None, class_logprobs(x, mask=mask), g_entropy=torch.ones(5, device="cuda"), mask=mask)
+            broken = mask is None or bool(keep[C - 2])
+            if mask is None:
+                assert bool(torch.isnan(d).all())
+            elif broken:
+                assert bool(torch.isnan(d[:, keep]).all()) and float(d[:, ~keep].float().abs().max()) == 0

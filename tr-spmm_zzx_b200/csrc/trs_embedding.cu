@@ -29,7 +29,7 @@ template <class TI, class TO, int VEC, int G, int ROWS, int PER, bool COPY>
 __global__ void __launch_bounds__(kLookupThreads) k_lookup(const TI* __restrict__ table, unsigned rows, unsigned stride,
                                                            const void* __restrict__ ids, int ids64, unsigned n, int pieces, float scale,
                                                            long long padding, TO* __restrict__ out, unsigned out_stride) {
-    const unsigned group = (blockIdx.x * kLookupThreads + threadIdx.x) / G, i0 = group * ROWS;
+    const unsigned i0 = (blockIdx.x * (kLookupThreads / G) + threadIdx.x / G) * ROWS;   // below 2^32 wherever a CTA is
     int c = threadIdx.x % G;
     if (i0 >= n) return;
     const TI* from[ROWS];
@@ -599,6 +599,8 @@ GradPlan grad_plan(long long n, long long rows, int F) {
     return p;
 }
 
+bool aligned(const void* p, int bytes) { return (uintptr_t)p % bytes == 0; }
+
 int check_sizes(long long rows, long long n, int F) {
     if (rows < 1 || n < 0 || F < 1) return TRS_E_ARG;
     if (rows > kMaxRows || n > kMaxIds || F > kMaxFeatures) return TRS_E_LIMIT;
@@ -639,6 +641,7 @@ extern "C" int trs_embedding(const void* table, int table_type, long long rows, 
     if (table_stride > kMaxStride || out_stride > kMaxStride) return TRS_E_LIMIT;
     if (n == 0) return TRS_OK;
     if (!table || !ids || !out) return TRS_E_ARG;
+    if (!aligned(table, type_bytes(table_type)) || !aligned(ids, ids64 ? 8 : 4) || !aligned(out, type_bytes(out_type))) return TRS_E_ARG;
     const int vec = elements_per_piece(F, table, table_type, table_stride, out, out_type, out_stride), pieces = F / vec;
     return with_type(table_type, [&](auto ti) {
         return with_type(out_type, [&](auto to) {
@@ -684,6 +687,7 @@ extern "C" int trs_embedding_grad(const void* grad, int grad_type, long long gra
     if (rc) return rc;
     if (!type_known(grad_type) || !type_known(out_type) || grad_stride < F || out_stride < F || !out) return TRS_E_ARG;
     if (n && (!grad || !ids)) return TRS_E_ARG;
+    if ((n && (!aligned(grad, type_bytes(grad_type)) || !aligned(ids, ids64 ? 8 : 4))) || !aligned(out, type_bytes(out_type))) return TRS_E_ARG;
     if (n == 0 && accumulate) return TRS_OK;
     const cudaStream_t st = (cudaStream_t)stream;
     GradPlan p;

@@ -722,7 +722,7 @@ __device__ __forceinline__ void write_own(const Backward& a, long long r, const 
         for (int k = 0; k < a.top; ++k)
             if (a.top_ids[r * a.top + k] == j) own += a.g_top[r * a.top + k];
     const float x = as_float(row.x[j]);
-    if ((row.mask && !row.mask[j]) || x == -INFINITY) return;   // stays 0
+    if ((row.mask && !row.mask[j]) || x == -INFINITY) return;   // as it is
     dx[j] = from_float<T>(a.scale * (own + without_own(g, x)));
 }
 template <class T>
@@ -738,7 +738,9 @@ __device__ __forceinline__ void write_piece(const Backward& a, const RowGrad& g,
         row.load(piece, v);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
-            const bool out = v[k] == -INFINITY;   // masked, or as good as
+            bool out = v[k] == -INFINITY;   // masked, or as good as
+            if (out && g.inv_S != g.inv_S)   // in a row without a distribution what is not masked is NaN
+                out = (unsigned)(j + k) >= (unsigned)row.classes || (row.mask && !row.mask[j + k]);
             q.v[k] = from_float<T>(out ? 0.f : a.scale * without_own(g, v[k]));
         }
     }
@@ -876,7 +878,7 @@ Extent extent(const void* p, long long rows, long long stride, long long width, 
 
 int check(const void* x, int type, long long n, int classes, long long stride, const void* mask, long long mask_stride, float scale,
           int top) {
-    if (!type_known(type) || n < 0 || classes < 1 || stride < classes || top < 0 || !(scale > 0.f) || !(scale < INFINITY)) return TRS_E_ARG;
+    if (!type_known(type) || n < 0 || classes < 1 || stride < classes || top < 0 || !(scale > 0.f) || !(scale * kLog2e < INFINITY)) return TRS_E_ARG;
     if (mask && mask_stride != 0 && mask_stride < classes) return TRS_E_ARG;
     if (n > 0x7fffffffll || classes > (1 << 30) || top > kMaxTop) return TRS_E_LIMIT;
     if (n && (!x || (uintptr_t)x % type_bytes(type))) return TRS_E_ARG;
@@ -894,7 +896,10 @@ extern "C" int trs_logprobs(const void* x, int type, long long n, int classes, l
     const int rc = check(x, type, n, classes, stride, mask, mask_stride, scale, top);
     if (rc) return rc;
     if (n == 0) return TRS_OK;
-    if ((logprobs && !targets) || (top && (!top_logprobs || !top_ids)) || (uintptr_t)stats % 8) return TRS_E_ARG;
+    if ((logprobs && (!targets || (uintptr_t)targets % (targets64 ? 8 : 4))) || ((uintptr_t)logprobs | (uintptr_t)entropy) % 4 ||
+        ((uintptr_t)top_logprobs | (uintptr_t)top_ids) % 4)
+        return TRS_E_ARG;
+    if ((top && (!top_logprobs || !top_ids)) || (uintptr_t)stats % 8) return TRS_E_ARG;
     const Forward a{x, n, stride, classes, targets, targets64, ignore_id, mask, mask_stride, extent(x, n, stride, classes, type_bytes(type)), extent(mask, n, mask_stride, classes, 1), scale, scale * kLog2e, top, logprobs, entropy,
                     top_logprobs, top_ids, (float2*)stats};
     return with_type(type, [&](auto t) {
@@ -931,7 +936,8 @@ extern "C" int trs_logprobs_grad(const void* x, int type, long long n, int class
     if (dx_stride < classes) return TRS_E_ARG;
     if (n == 0) return TRS_OK;
     if (!dx || (uintptr_t)dx % type_bytes(type) || !stats || (uintptr_t)stats % 8) return TRS_E_ARG;
-    if ((g_logprobs && !targets) || (g_entropy && !entropy) || (g_top_logprobs && (!top_ids || !top))) return TRS_E_ARG;
+    if (((uintptr_t)entropy | (uintptr_t)g_logprobs | (uintptr_t)g_entropy | (uintptr_t)g_top_logprobs | (uintptr_t)top_ids) % 4) return TRS_E_ARG;
+    if ((g_logprobs && (!targets || (uintptr_t)targets % (targets64 ? 8 : 4))) || (g_entropy && !entropy) || (g_top_logprobs && (!top_ids || !top))) return TRS_E_ARG;
     const Backward a{x, n, stride, classes, targets, targets64, ignore_id, mask, mask_stride, extent(x, n, stride, classes, type_bytes(type)), extent(mask, n, mask_stride, classes, 1), scale, scale * kLog2e, top, top_ids,
                      (const float2*)stats, entropy, g_logprobs, g_entropy, g_top_logprobs, dx, dx_stride};
     return with_type(type, [&](auto t) {
