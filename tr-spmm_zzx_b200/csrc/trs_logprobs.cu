@@ -84,9 +84,12 @@ struct Row {
     Extent x_in, mask_in;
     template <class Args>
     __device__ __forceinline__ Row(const Args& a, long long r) : classes(a.classes), x_in(a.x_in), mask_in(a.mask_in) {
-        x = (const T*)a.x + r * a.stride;
-        mask = a.mask ? a.mask + r * a.mask_stride : nullptr;
-        head = (int)((uintptr_t)x % 16 / sizeof(T));
+        at((const T*)a.x + r * a.stride, a.mask ? a.mask + r * a.mask_stride : nullptr);
+    }
+    __device__ __forceinline__ void at(const T* x_, const unsigned char* mask_) {
+        x = x_;
+        mask = mask_;
+        head = (int)((unsigned)(uintptr_t)x % 16 / sizeof(T));
         pieces = (head + classes + VEC - 1) / VEC;
     }
     __device__ __forceinline__ int first(int piece) const { return piece * VEC - head; }
@@ -231,7 +234,8 @@ __device__ __forceinline__ Key warp_sort(Key k) {
 // second largest of its pieces' maxima reaches K too - and the few scores that reach K are put in order by their ranks.
 //
 // Few rows are split over the CTAs of a cluster (`parts`), which hand their sums and alternatives to the first one.
-constexpr int kCandidates = 1024, kTurn = 4, kMaxParts = 8;
+constexpr int kTurn = 4, kMaxParts = 8;
+constexpr int candidates(int threads) { return threads >= 128 ? 1024 : 256; }   // (the alternatives of 8 parts fit)
 
 // A thread's sums with two accumulators, relative to `ref`: a maximum up to 2^kSlack below the present one (e^(d) stays far from
 // overflow, and sums are rescaled once or twice in a row instead of at every new maximum); and where the maximum is first.
@@ -274,7 +278,7 @@ struct Running {
     }
 };
 template <class T, int THREADS, bool MASKED>
-__global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_row(const Forward a, int parts) {
+__global__ void __launch_bounds__(THREADS, THREADS == 32 ? 24 : 1280 / THREADS) k_row(const Forward a, int parts) {
     constexpr int WARPS = THREADS / 32, VEC = Row<T>::VEC, TURN = kTurn, WORDS = VEC / 4 + 1;
     const long long r = blockIdx.x / parts;
     const int part = (int)(blockIdx.x - r * parts);
@@ -398,7 +402,7 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_row(const Forward a
         s.template add<false>(x, make_float2(-s.ref, -s.ref), c2);
     }
     __shared__ Sums s_part[WARPS], s_all;
-    __shared__ Key s_key[THREADS], s_found[kCandidates], s_best[kMaxTop];
+    __shared__ Key s_key[THREADS], s_found[candidates(THREADS)], s_best[kMaxTop];
     __shared__ Key s_bound;
     __shared__ int s_sel[THREADS], s_count[2];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -445,7 +449,7 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_row(const Forward a
                 const Key key = key_of(v[k], row.first(piece) + k);
                 if (key < bound) continue;
                 const int to = atomicAdd(&s_count[1], 1);
-                if (to < kCandidates) s_found[to] = key;
+                if (to < candidates(THREADS)) s_found[to] = key;
             }
         };
         if (some && key_of(s.m, max(row.first(s.at), 0)) >= bound) {
@@ -489,7 +493,7 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_row(const Forward a
         __syncthreads();
         if (s_count[1] <= 256) {
             rank_top(s_found, s_count[1], a.top, s_best, threadIdx.x, THREADS);
-        } else if (s_count[1] <= kCandidates) {
+        } else if (s_count[1] <= candidates(THREADS)) {
             if (warp == 0) warp_top(s_found, s_count[1], a.top, s_best);
         } else {
             // more scores than the list holds (rows in which a few threads' parts have nearly all of the largest ones): one round
@@ -557,41 +561,11 @@ __device__ __forceinline__ Sums group_sum(Sums s) {   // m is common
     return s;
 }
 
+// The alternatives of a row that a group of lanes holds.
 template <class T, int G, int PER>
-__global__ void __launch_bounds__(kShortThreads) k_short_rows(const Forward a) {
+__device__ __forceinline__ void short_top(const Forward& a, long long r, const Row<T>& row, float (&v)[PER][Row<T>::VEC], const Sums& s) {
     constexpr int VEC = Row<T>::VEC;
     const int g = threadIdx.x % G;
-    const long long r0 = ((long long)blockIdx.x * kShortThreads + threadIdx.x) / G, r = r0 < a.n ? r0 : a.n - 1;   // lanes stay together
-    const Row<T> row(a, r);
-    float v[PER][VEC];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        if (g + i * G < row.pieces) {
-            row.load(g + i * G, v[i]);
-        } else {
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) v[i][k] = -INFINITY;
-        }
-    }
-    float m = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) m = max_nan(m, v[i][k]);
-#pragma unroll
-    for (int o = G / 2; o; o /= 2) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-    Sums s{m, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-            const float d = fmaxf((v[i][k] - m) * a.c, kFar), e = exp_2(d);
-            s.S += e;
-            s.T = fmaf(e, d, s.T);
-        }
-    s = group_sum<G>(s);
-    if (g == 0 && r == r0) write_row<T>(a, r, row.x, row.mask, s);
-    if (!a.top) return;
     const float log_S = logf(s.S);
     // One word a score: as much of its order as fits above its class, so that a maximum of words is a maximum of scores with the lowest
     // class first among equal ones.  16-bit scores fit; fp32 scores lose their lowest bits, and where two of the best (or the
@@ -624,14 +598,16 @@ __global__ void __launch_bounds__(kShortThreads) k_short_rows(const Forward a) {
         if (k >= a.top) break;
         if (k % G == g) mine = found;
         if (k % G == G - 1 || k == a.top - 1) {
-            if (g <= k % G && r == r0) {
+            if (g <= k % G && r < a.n) {
                 const int id = (int)(low - (mine & low));
                 write_top(a, r, k - k % G + g, mine != 0, id, mine ? as_float(row.x[id]) : 0.f, s.m, log_S);
             }
         }
     }
-    if (sizeof(T) == 2 || !__any_sync(0xffffffffu, close)) return;
+    if constexpr (sizeof(T) == 4) {
+    if (!__any_sync(0xffffffffu, close)) return;
     for (int k = 0; k < a.top; ++k) {
+        float m = s.m;
         if (k) {
             m = -INFINITY;
 #pragma unroll
@@ -654,7 +630,62 @@ __global__ void __launch_bounds__(kShortThreads) k_short_rows(const Forward a) {
 #pragma unroll
             for (int q = 0; q < VEC; ++q)
                 if (row.first(g + i * G) + q == at) v[i][q] = -INFINITY;
-        if (k % G == g && r == r0) write_top(a, r, k, m > -INFINITY, at, m, s.m, log_S);
+        if (k % G == g && r < a.n) write_top(a, r, k, m > -INFINITY, at, m, s.m, log_S);
+    }
+    }
+}
+
+// A group does ROWS rows one after the other, and a lane each of what is to be done once a row (ROWS = 1 where rows are few).
+template <class T, int G, int PER, int ROWS>
+__global__ void __launch_bounds__(kShortThreads) k_short_rows(const Forward a) {
+    static_assert(ROWS == 1 || ROWS <= G, "a lane a row");
+    constexpr int VEC = Row<T>::VEC;
+    const int g = threadIdx.x % G;
+    const long long r0 = ((long long)blockIdx.x * (kShortThreads / G) + threadIdx.x / G) * ROWS;
+    Row<T> row(a, min(r0, a.n - 1));   // (groups past the end do the last row once more, and write nothing: lanes stay together)
+    Sums own{};                        // of row r0 + g
+    const float2 c2 = make_float2(a.c, a.c);
+#pragma unroll 1
+    for (int u = 0; u < ROWS; ++u) {
+        const long long r = r0 + u;
+        if (u && r < a.n) row.at(row.x + a.stride, row.mask ? row.mask + a.mask_stride : nullptr);
+        float v[PER][VEC];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if (g + i * G < row.pieces) {
+                row.load(g + i * G, v[i]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) v[i][k] = -INFINITY;
+            }
+        }
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+#pragma unroll
+            for (int k = 0; k < VEC; k += 2) m = max_nan(m, v[i][k], v[i][k + 1]);
+#pragma unroll
+        for (int o = G / 2; o; o /= 2) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float2 minus = make_float2(-m, -m);
+        float2 S = make_float2(0.f, 0.f), Q = S;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+#pragma unroll
+            for (int k = 0; k < VEC; k += 2) {
+                float2 d = __fmul2_rn(__fadd2_rn(make_float2(v[i][k], v[i][k + 1]), minus), c2);
+                d.x = fmaxf(d.x, kFar);
+                d.y = fmaxf(d.y, kFar);
+                const float2 e = make_float2(exp_2(d.x), exp_2(d.y));
+                S = __fadd2_rn(S, e);
+                Q = __ffma2_rn(e, d, Q);
+            }
+        const Sums s = group_sum<G>(Sums{m, S.x + S.y, Q.x + Q.y});
+        if (u == g) own = s;
+        if (a.top) short_top<T, G, PER>(a, r, row, v, s);
+    }
+    if (g < ROWS && r0 + g < a.n) {
+        row.at((const T*)a.x + (r0 + g) * a.stride, a.mask ? a.mask + (r0 + g) * a.mask_stride : nullptr);
+        write_row<T>(a, r0 + g, row.x, row.mask, own);
     }
 }
 
@@ -725,6 +756,13 @@ __device__ __forceinline__ void write_own(const Backward& a, long long r, const 
     if ((row.mask && !row.mask[j]) || x == -INFINITY) return;   // as it is
     dx[j] = from_float<T>(a.scale * (own + without_own(g, x)));
 }
+// The k-th of the classes with weights: the target, then the alternatives.
+template <class T>
+__device__ __forceinline__ void write_own_of(const Backward& a, long long r, const RowGrad& g, const Row<T>& row, int k) {
+    const long long j = k ? a.top_ids[r * a.top + k - 1] : a.g_logprobs ? load_target(a.target, a.target64, r) : -1;
+    if (j < 0 || j >= a.classes || (k == 0 && !target_counts(a, j))) return;
+    write_own<T>(a, r, g, row, (T*)a.dx + r * a.dx_stride, j);
+}
 template <class T>
 __device__ __forceinline__ void write_piece(const Backward& a, const RowGrad& g, const Row<T>& row, T* dx, int piece) {
     constexpr int VEC = Row<T>::VEC;
@@ -753,10 +791,10 @@ __device__ __forceinline__ void write_piece(const Backward& a, const RowGrad& g,
     }
 }
 
-constexpr int kGradThreads = 256, kGradTurn = 4, kGradPieces = 2 * kGradTurn;   // pieces per thread: turns of four whose loads are under way together
+constexpr int kGradTurn = 4, kGradPieces = 2 * kGradTurn;   // pieces per thread: turns of four whose loads are under way together
 
-template <class T, bool MASKED>
-__global__ void __launch_bounds__(kGradThreads) k_row_grad(const Backward a, int parts) {
+template <class T, int THREADS, bool MASKED>
+__global__ void __launch_bounds__(THREADS) k_row_grad(const Backward a, int parts) {
     constexpr int VEC = Row<T>::VEC;
     const long long r = blockIdx.x / parts;
     const int part = (int)(blockIdx.x - r * parts);
@@ -768,21 +806,21 @@ __global__ void __launch_bounds__(kGradThreads) k_row_grad(const Backward a, int
     const bool straight = (uintptr_t)(dx - row.head) % 16 == 0;
     const int q0 = straight && !MASKED ? max(p0, row.head ? 1 : 0) : p1, q1 = min(p1, (row.head + row.classes) / VEC);
     if (g.zero) {
-        for (int piece = p0 + threadIdx.x; piece < p1; piece += kGradThreads) write_piece<T>(a, g, row, dx, piece);
+        for (int piece = p0 + threadIdx.x; piece < p1; piece += THREADS) write_piece<T>(a, g, row, dx, piece);
         return;
     }
     const float2 minus = make_float2(-g.m, -g.m), c2 = make_float2(g.c, g.c), A2 = make_float2(g.A, g.A), B2 = make_float2(g.B, g.B);
     const float f = -a.scale * g.inv_S * (g.B != 0.f ? 1.f : g.A);
     const float2 f2 = make_float2(f, f);
     auto whole = [&](auto with_d) {
-        for (int base = q0 + threadIdx.x; base < q1; base += kGradTurn * kGradThreads) {
+        for (int base = q0 + threadIdx.x; base < q1; base += kGradTurn * THREADS) {
             Piece<T, VEC> w[kGradTurn];
 #pragma unroll
             for (int u = 0; u < kGradTurn; ++u)
-                if (base + u * kGradThreads < q1) w[u] = *(const Piece<T, VEC>*)(row.x + row.first(base + u * kGradThreads));
+                if (base + u * THREADS < q1) w[u] = *(const Piece<T, VEC>*)(row.x + row.first(base + u * THREADS));
 #pragma unroll
             for (int u = 0; u < kGradTurn; ++u) {
-                if (base + u * kGradThreads >= q1) break;
+                if (base + u * THREADS >= q1) break;
                 float v[VEC];
                 as_floats(w[u], v);
                 Piece<T, VEC> q;
@@ -798,17 +836,17 @@ __global__ void __launch_bounds__(kGradThreads) k_row_grad(const Backward a, int
                     q.v[k] = from_float<T>(y.x);
                     q.v[k + 1] = from_float<T>(y.y);
                 }
-                *(Piece<T, VEC>*)(dx + row.first(base + u * kGradThreads)) = q;
+                *(Piece<T, VEC>*)(dx + row.first(base + u * THREADS)) = q;
             }
         }
     };
     if (g.B != 0.f) whole(std::true_type());
     else whole(std::false_type());   // the weight is A for all
     // the others: those that the row's ends cut, or all
-    for (int piece = p0 + threadIdx.x; piece < min(q0, p1); piece += kGradThreads) write_piece<T>(a, g, row, dx, piece);
-    for (int piece = max(q0, q1) + threadIdx.x; piece < p1; piece += kGradThreads) write_piece<T>(a, g, row, dx, piece);
+    for (int piece = p0 + threadIdx.x; piece < min(q0, p1); piece += THREADS) write_piece<T>(a, g, row, dx, piece);
+    for (int piece = max(q0, q1) + threadIdx.x; piece < p1; piece += THREADS) write_piece<T>(a, g, row, dx, piece);
     __syncthreads();   // classes with weights of their own are written once more, by one thread each (equal values where they coincide)
-    for (int k = threadIdx.x; k < 1 + (a.g_top ? a.top : 0); k += kGradThreads) {
+    for (int k = threadIdx.x; k < 1 + (a.g_top ? a.top : 0); k += THREADS) {
         const long long j = k ? a.top_ids[r * a.top + k - 1] : a.g_logprobs ? load_target(a.target, a.target64, r) : -1;
         if (j < 0 || j >= a.classes || (k == 0 && !target_counts(a, j))) continue;
         const int piece = (int)((j + row.head) / VEC);
@@ -816,41 +854,68 @@ __global__ void __launch_bounds__(kGradThreads) k_row_grad(const Backward a, int
     }
 }
 
-template <class T, int G, int PER>
+// A group does ROWS rows one after the other; what a row needs beside its scores is a lane's to fetch, and to write what has weights of its own.
+template <class T, int G, int PER, int ROWS>
 __global__ void __launch_bounds__(kShortThreads) k_short_rows_grad(const Backward a) {
+    static_assert(ROWS == 1 || ROWS <= G, "a lane a row");
     const int g = threadIdx.x % G;
-    const long long r = ((long long)blockIdx.x * kShortThreads + threadIdx.x) / G;
-    const bool in = r < a.n;
-    const Row<T> row(a, in ? r : 0);
-    T* dx = (T*)a.dx + (in ? r : 0) * a.dx_stride;
-    const RowGrad w = row_grad(a, in ? r : 0);
+    const long long r0 = ((long long)blockIdx.x * (kShortThreads / G) + threadIdx.x / G) * ROWS;
+    const long long mine = min(r0 + (ROWS == 1 ? 0 : g % ROWS), a.n - 1);
+    const RowGrad own = row_grad(a, mine);
+    Row<T> row(a, min(r0, a.n - 1));
+    T* dx = (T*)a.dx + min(r0, a.n - 1) * a.dx_stride;
+#pragma unroll 1
+    for (int u = 0; u < ROWS; ++u) {
+        RowGrad w = own;
+        if (ROWS > 1) {
+            w.m = __shfl_sync(0xffffffffu, own.m, u, G);
+            w.inv_S = __shfl_sync(0xffffffffu, own.inv_S, u, G);
+            w.A = __shfl_sync(0xffffffffu, own.A, u, G);
+            w.B = __shfl_sync(0xffffffffu, own.B, u, G);
+            w.zero = __shfl_sync(0xffffffffu, (int)own.zero, u, G);
+        }
+        if (r0 + u < a.n) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-        if (in && g + i * G < row.pieces) write_piece<T>(a, w, row, dx, g + i * G);
+            for (int i = 0; i < PER; ++i)
+                if (g + i * G < row.pieces) write_piece<T>(a, w, row, dx, g + i * G);
+            row.at(row.x + a.stride, row.mask ? row.mask + a.mask_stride : nullptr);   // (only looked at where there is a next row)
+            dx += a.dx_stride;
+        }
+    }
     __syncwarp();   // behind the lanes of the row, as in k_row_grad
-    if (!in || w.zero) return;
-    for (int k = g; k < 1 + (a.g_top ? a.top : 0); k += G) {
-        const long long j = k ? a.top_ids[r * a.top + k - 1] : a.g_logprobs ? load_target(a.target, a.target64, r) : -1;
-        if (j < 0 || j >= a.classes || (k == 0 && !target_counts(a, j))) continue;
-        write_own<T>(a, r, w, row, dx, j);
+    if (ROWS > 1) {
+        if (g >= ROWS || r0 + g >= a.n || own.zero) return;
+        const Row<T> its(a, mine);
+        for (int k = 0; k < 1 + (a.g_top ? a.top : 0); ++k) write_own_of<T>(a, mine, own, its, k);
+    } else {
+        if (r0 >= a.n || own.zero) return;
+        const Row<T> its(a, mine);
+        for (int k = g; k < 1 + (a.g_top ? a.top : 0); k += G) write_own_of<T>(a, mine, own, its, k);
     }
 }
 
-// Lanes and pieces per lane that hold a row of so many pieces; beyond 32 x 2 x (16 scores) a row is a CTA's.
-constexpr int kShortScores = 16;
+// Lanes and pieces per lane that hold a row of so many pieces, and rows a group.  Longer ones are a CTA's: forward from 128 pieces on, the
+// gradient from 64 (2^27 fp16 scores, us: 1000 classes 136 by groups, 148 by CTAs; their gradient 194, 119; of 300 classes 379, 392).
+constexpr int kShortScores = 16, kShortPieces = 128, kShortPiecesGrad = 64;
 template <class T, class Fn>
-int with_short(int pieces, Fn fn) {
+int with_short(int pieces, long long n, Fn fn) {
     constexpr int PER = kShortScores / Row<T>::VEC;
-    if (pieces <= PER) return fn(std::integral_constant<int, 1>(), std::integral_constant<int, PER>());
-    if (pieces <= 2 * PER) return fn(std::integral_constant<int, 2>(), std::integral_constant<int, PER>());
-    if (pieces <= 4 * PER) return fn(std::integral_constant<int, 4>(), std::integral_constant<int, PER>());
-    if (pieces <= 8 * PER) return fn(std::integral_constant<int, 8>(), std::integral_constant<int, PER>());
-    if (pieces <= 16 * PER) return fn(std::integral_constant<int, 16>(), std::integral_constant<int, PER>());
-    if (pieces <= 32 * PER) return fn(std::integral_constant<int, 32>(), std::integral_constant<int, PER>());
-    return fn(std::integral_constant<int, 32>(), std::integral_constant<int, 2 * PER>());
+    auto rows = [&](auto g, auto per) {
+        constexpr int G = decltype(g)::value, ROWS = G < 8 ? G : 8;
+        if (ROWS > 1 && n * G / ROWS >= 4 * 148 * 1024) return fn(g, per, std::integral_constant<int, ROWS>());   // otherwise more lanes are worth more
+        return fn(g, per, std::integral_constant<int, 1>());
+    };
+    const std::integral_constant<int, PER> per;
+    if (pieces <= PER) return rows(std::integral_constant<int, 1>(), per);
+    if (pieces <= 2 * PER) return rows(std::integral_constant<int, 2>(), per);
+    if (pieces <= 4 * PER) return rows(std::integral_constant<int, 4>(), per);
+    if (pieces <= 8 * PER) return rows(std::integral_constant<int, 8>(), per);
+    if (pieces <= 16 * PER) return rows(std::integral_constant<int, 16>(), per);
+    if constexpr (32 * PER < kShortPieces) {
+        if (pieces > 32 * PER) return rows(std::integral_constant<int, 32>(), std::integral_constant<int, 2 * PER>());
+    }
+    return rows(std::integral_constant<int, 32>(), per);
 }
-template <class T>
-constexpr int kShortPieces = 64 * kShortScores / Row<T>::VEC;
 // Pieces of a row, wherever it begins.
 template <class T>
 int most_pieces(int classes) { return (int)ceil_div64((long long)classes + Row<T>::VEC - 1, Row<T>::VEC); }
@@ -905,19 +970,26 @@ extern "C" int trs_logprobs(const void* x, int type, long long n, int classes, l
     return with_type(type, [&](auto t) {
         using T = decltype(t);
         const int pieces = most_pieces<T>(classes);
-        if (pieces <= kShortPieces<T>)
-            return with_short<T>(pieces, [&](auto g, auto per) {
-                constexpr int G = decltype(g)::value;
-                return launch(k_short_rows<T, G, decltype(per)::value>, dim3((unsigned)ceil_div64(n * G, kShortThreads)), kShortThreads, 0,
-                              (cudaStream_t)stream, a);
+        if (pieces <= kShortPieces)
+            return with_short<T>(pieces, n, [&](auto g, auto per, auto rows) {
+                constexpr int G = decltype(g)::value, ROWS = decltype(rows)::value;
+                return launch(k_short_rows<T, G, decltype(per)::value, ROWS>, dim3((unsigned)ceil_div64(ceil_div64(n, ROWS) * G, kShortThreads)),
+                              kShortThreads, 0, (cudaStream_t)stream, a);
             });
         auto run = [&](auto threads, int parts) {
             constexpr int THREADS = decltype(threads)::value;
             return a.mask ? launch_rows<T, THREADS, true>(n, parts, (cudaStream_t)stream, a)
                           : launch_rows<T, THREADS, false>(n, parts, (cudaStream_t)stream, a);
         };
-        if (pieces <= 128 * kTurn) return run(std::integral_constant<int, 128>(), 1);
-        // Few rows: parts until there are two CTAs an SM (or a part has one turn).  More of them only add ends: 512 rows of 2^18 masked
+        // As few threads a row as keep it going, many rows at a time: what a row costs beside its scores grows with its threads.  2^27 fp16
+        // scores by 32 / 64 / 128 / 256 threads, us: 2000 classes 99 / 122 / 146 / 247, 9000: 67 / 56 / 62 / 87, 33000:
+        // 70 / 54 / 52 / 56; fp32 33000: 89 / 99 / 93 / 97.
+        int threads = sizeof(T) == 4 ? (pieces <= 8192 ? 32 : 256) : pieces <= 640 ? 32 : pieces <= 2400 ? 64 : pieces <= 8192 ? 128 : 256;
+        while (threads < 256 && n * threads < 148 * 1024 && pieces > threads * kTurn) threads *= 2;   // unless rows are few
+        if (threads == 32) return run(std::integral_constant<int, 32>(), 1);
+        if (threads == 64) return run(std::integral_constant<int, 64>(), 1);
+        if (threads == 128) return run(std::integral_constant<int, 128>(), 1);
+        // Very few rows: parts until there are two CTAs an SM (or a part has one turn).  More of them only add ends: 512 rows of 2^18 masked
         // fp16 scores, ten alternatives: 87 us whole, 92 / 96 / 125 us in 2 / 4 / 8 parts.
         int parts = 1;
         while (parts < kMaxParts && n * parts < 2 * 148 && pieces > parts * 256 * kTurn) parts *= 2;
@@ -943,16 +1015,22 @@ extern "C" int trs_logprobs_grad(const void* x, int type, long long n, int class
     return with_type(type, [&](auto t) {
         using T = decltype(t);
         const int pieces = most_pieces<T>(classes);
-        if (pieces <= kShortPieces<T>)
-            return with_short<T>(pieces, [&](auto g, auto per) {
-                constexpr int G = decltype(g)::value;
-                return launch(k_short_rows_grad<T, G, decltype(per)::value>, dim3((unsigned)ceil_div64(n * G, kShortThreads)), kShortThreads,
-                              0, (cudaStream_t)stream, a);
+        if (pieces <= kShortPiecesGrad)
+            return with_short<T>(pieces, n, [&](auto g, auto per, auto rows) {
+                constexpr int G = decltype(g)::value, ROWS = decltype(rows)::value;
+                return launch(k_short_rows_grad<T, G, decltype(per)::value, ROWS>,
+                              dim3((unsigned)ceil_div64(ceil_div64(n, ROWS) * G, kShortThreads)), kShortThreads, 0, (cudaStream_t)stream, a);
             });
-        const long long parts = ceil_div64((long long)classes + Row<T>::VEC - 1, (long long)Row<T>::VEC * kGradThreads * kGradPieces);
-        if (n * parts > 0x7fffffffll) return (int)TRS_E_LIMIT;
-        return launch(a.mask ? k_row_grad<T, true> : k_row_grad<T, false>, dim3((unsigned)(n * parts)), kGradThreads, 0, (cudaStream_t)stream, a,
-                      (int)parts);
+        auto run = [&](auto threads) {
+            constexpr int THREADS = decltype(threads)::value;
+            const long long parts = ceil_div64(pieces, THREADS * kGradPieces);
+            if (n * parts > 0x7fffffffll) return (int)TRS_E_LIMIT;
+            return launch(a.mask ? k_row_grad<T, THREADS, true> : k_row_grad<T, THREADS, false>, dim3((unsigned)(n * parts)), THREADS, 0,
+                          (cudaStream_t)stream, a, (int)parts);
+        };
+        // (2^27 fp16 scores by 32 / 64 / 256 threads, us: 1100 classes 144 / 195 / 525, 9000: 98 / 93 / 107, 33000: 94 / 88 / 99)
+        if (pieces <= 32 * kGradPieces) return run(std::integral_constant<int, 32>());
+        return run(std::integral_constant<int, 64>());
     });
 }
 TRS_CATCH
