@@ -26,7 +26,7 @@ __device__ __forceinline__ long long load_id(const void* __restrict__ ids, int i
 constexpr int kThreads = 256, kLookupThreads = 128;
 
 template <class TI, class TO, int VEC, int G, int ROWS, int PER, bool COPY>
-__global__ void __launch_bounds__(kLookupThreads) k_lookup(const TI* __restrict__ table, unsigned rows, unsigned stride,
+__global__ void __launch_bounds__(kLookupThreads, 8) k_lookup(const TI* __restrict__ table, unsigned rows, unsigned stride,
                                                            const void* __restrict__ ids, int ids64, unsigned n, int pieces, float scale,
                                                            long long padding, TO* __restrict__ out, unsigned out_stride) {
     const unsigned i0 = (blockIdx.x * (kLookupThreads / G) + threadIdx.x / G) * ROWS;   // below 2^32 wherever a CTA is

@@ -4,7 +4,7 @@ The features of a graph whose nodes have none of their own are a learned table, 
     out[i, :]  = scale * table[ids[i], :]
     grad[v, :] = scale * sum of dout[i, :] over the i with ids[i] = v
 which are the products with the selection matrix of the ids and with its transpose.  The reference has neither (its
-dataset classes draw random features, spmm/tr_csr_fp16/mdataset2_online.py:98-101).
+dataset classes draw random features, spmm/tr_csr_fp16/mdataset2_online.py:29-167).
 """
 from __future__ import annotations
 
