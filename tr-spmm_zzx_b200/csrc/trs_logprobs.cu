@@ -131,6 +131,40 @@ struct Row {
     }
 };
 
+// The mask's bytes of whole pieces, out of the aligned words that hold them.
+template <int VEC>
+struct MaskWords {
+    static constexpr int WORDS = VEC / 4 + 1;
+    const unsigned char* word;   // of piece 0
+    unsigned shift;
+    int last;                    // the last word with a byte of the piece
+    bool even;                   // a piece's bytes in one load
+    __device__ __forceinline__ MaskWords(const unsigned char* mask, int head) {
+        const uintptr_t at = (uintptr_t)(mask - head);
+        word = (const unsigned char*)(at & ~(uintptr_t)3);
+        shift = ((unsigned)at & 3) * 8;
+        last = shift ? VEC : VEC - 4;
+        even = at % VEC == 0;
+    }
+    __device__ __forceinline__ void fetch(unsigned (&bits)[WORDS], int piece) const {
+        const unsigned char* w = word + (size_t)piece * VEC;
+        if (even) {
+            const Piece<unsigned, VEC / 4> b = *(const Piece<unsigned, VEC / 4>*)w;
+#pragma unroll
+            for (int k = 0; k < VEC / 4; ++k) bits[k] = b.v[k];
+            bits[VEC / 4] = 0;
+        } else {
+#pragma unroll
+            for (int k = 0; k < WORDS; ++k) bits[k] = __ldg((const unsigned*)(w + (k < WORDS - 1 ? 4 * k : last)));
+        }
+    }
+    template <class T>
+    __device__ __forceinline__ void apply(Piece<T, VEC>& x, const unsigned (&bits)[WORDS]) const {   // -inf where masked
+#pragma unroll
+        for (int k = 0; k < VEC / 4; ++k) mask_four(x, 4 * k, __funnelshift_r(bits[k], bits[k + 1], shift));
+    }
+};
+
 struct Forward {
     const void* x;
     long long n, stride;
@@ -287,45 +321,23 @@ __global__ void __launch_bounds__(THREADS, THREADS == 32 ? 24 : 1280 / THREADS) 
     // pieces [q0, q1) lie inside the row
     int q0 = max(p0, row.head ? 1 : 0);
     int q1 = min(p1, (row.head + row.classes) / VEC);
-    const unsigned char* mask_word = nullptr;
-    unsigned mask_shift = 0;
-    if (MASKED) {
-        mask_word = (const unsigned char*)((uintptr_t)(row.mask - row.head) & ~(uintptr_t)3);
-        mask_shift = ((uintptr_t)(row.mask - row.head) & 3) * 8;
-    }
-    const bool mask_even = MASKED && (uintptr_t)(row.mask - row.head) % VEC == 0;   // a piece's bytes in one load
-    const int last_word = mask_shift ? VEC : VEC - 4;   // the last word with a byte of the piece
     q0 = min(q0, p1);
     q1 = max(q1, q0);
+    const MaskWords<VEC> mask(row.mask, row.head);
     const float2 c2 = make_float2(a.c, a.c);
     Running s;
     struct Raw {
         Piece<T, VEC> x;
         unsigned bits[WORDS];
     };
-    auto fetch_mask = [&](Raw& w, int piece) {
-        if (MASKED && mask_even) {
-            const Piece<unsigned, VEC / 4> b = *(const Piece<unsigned, VEC / 4>*)(mask_word + (size_t)piece * VEC);
-#pragma unroll
-            for (int k = 0; k < VEC / 4; ++k) w.bits[k] = b.v[k];
-            w.bits[VEC / 4] = 0;
-        } else if (MASKED) {
-#pragma unroll
-            for (int k = 0; k < WORDS; ++k)
-                w.bits[k] = __ldg((const unsigned*)(mask_word + (size_t)piece * VEC + (k < WORDS - 1 ? 4 * k : last_word)));
-        }
-    };
     auto fetch = [&](int piece) {
         Raw w;
         w.x = *(const Piece<T, VEC>*)(row.x + row.first(piece));
-        fetch_mask(w, piece);
+        if (MASKED) mask.fetch(w.bits, piece);
         return w;
     };
     auto masked = [&](Raw& w) {
-        if (MASKED) {
-#pragma unroll
-            for (int k = 0; k < VEC / 4; ++k) mask_four(w.x, 4 * k, __funnelshift_r(w.bits[k], w.bits[k + 1], mask_shift));
-        }
+        if (MASKED) mask.apply(w.x, w.bits);
     };
     // one turn; `near`: no difference is bounded, and the answer is whether none needed to be (otherwise nothing is added)
     auto take = [&](auto near, int base) {
@@ -804,7 +816,8 @@ __global__ void __launch_bounds__(THREADS) k_row_grad(const Backward a, int part
     const int per = (row.pieces + parts - 1) / parts, p0 = min(row.pieces, part * per), p1 = min(row.pieces, p0 + per);
     // whole pieces whose places in dx are aligned as in x
     const bool straight = (uintptr_t)(dx - row.head) % 16 == 0;
-    const int q0 = straight && !MASKED ? max(p0, row.head ? 1 : 0) : p1, q1 = min(p1, (row.head + row.classes) / VEC);
+    const bool broken = MASKED && g.inv_S != g.inv_S;   // what is masked is 0 even there: piece by piece
+    const int q0 = straight && !broken ? max(p0, row.head ? 1 : 0) : p1, q1 = min(p1, (row.head + row.classes) / VEC);
     if (g.zero) {
         for (int piece = p0 + threadIdx.x; piece < p1; piece += THREADS) write_piece<T>(a, g, row, dx, piece);
         return;
@@ -812,15 +825,21 @@ __global__ void __launch_bounds__(THREADS) k_row_grad(const Backward a, int part
     const float2 minus = make_float2(-g.m, -g.m), c2 = make_float2(g.c, g.c), A2 = make_float2(g.A, g.A), B2 = make_float2(g.B, g.B);
     const float f = -a.scale * g.inv_S * (g.B != 0.f ? 1.f : g.A);
     const float2 f2 = make_float2(f, f);
+    const MaskWords<VEC> mask(row.mask, row.head);
     auto whole = [&](auto with_d) {
         for (int base = q0 + threadIdx.x; base < q1; base += kGradTurn * THREADS) {
             Piece<T, VEC> w[kGradTurn];
+            unsigned bits[kGradTurn][MaskWords<VEC>::WORDS];
 #pragma unroll
             for (int u = 0; u < kGradTurn; ++u)
-                if (base + u * THREADS < q1) w[u] = *(const Piece<T, VEC>*)(row.x + row.first(base + u * THREADS));
+                if (base + u * THREADS < q1) {
+                    w[u] = *(const Piece<T, VEC>*)(row.x + row.first(base + u * THREADS));
+                    if (MASKED) mask.fetch(bits[u], base + u * THREADS);
+                }
 #pragma unroll
             for (int u = 0; u < kGradTurn; ++u) {
                 if (base + u * THREADS >= q1) break;
+                if (MASKED) mask.apply(w[u], bits[u]);
                 float v[VEC];
                 as_floats(w[u], v);
                 Piece<T, VEC> q;
