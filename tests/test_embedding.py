@@ -207,6 +207,17 @@ def test_grad_sizes(rows, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 300, 70001, (1 << 20), (1 << 22) + 3, (1 << 24) + 1])
+@pytest.mark.parametrize("n", [(1 << 19) - 1, 1 << 19, 600_011])
+def test_grad_of_many_ids(rows, n):
+    """One to four passes of narrow digits, and the last length that takes wide ones."""
+    from trspmm import embedding_grad
+    ids, g = _ids(n, rows, seed=n, skew=rows > 1000), _randn(n, 4, seed=2)
+    ref, extra = _grad_ref(g, ids, rows, 1.0)
+    _within(embedding_grad(g, ids, rows), ref, extra, F32)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("pattern", ["one row", "two rows", "sorted", "reversed", "runs", "last row"])
 @pytest.mark.parametrize("n", [300, 9000, 600_011])
 def test_grad_popular_rows(pattern, n):

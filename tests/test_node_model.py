@@ -100,3 +100,48 @@ def test_first_order_gradients_under_create_graph_and_no_second_order():
     assert g.shape == want.shape
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.sum(), W)
+
+
+@pytest.mark.parametrize("top", [0, 3])
+def test_entropy_alone_without_targets(top):
+    """Outputs that are None beside one that has a gradient."""
+    from trspmm import class_logprobs, class_logprobs_grad
+    x = torch.randn(20, 33, device="cuda", requires_grad=True)
+    r = class_logprobs(x, top=top)
+    assert r.logprobs is None and (r.top_ids is None) == (top == 0)
+    r.entropy.sum().backward()
+    lp = torch.log_softmax(x.detach().double(), 1)
+    H = -(lp.exp() * lp).sum(1, keepdim=True)
+    want = -lp.exp() * (lp + H)
+    # p, log p and H are off by a few 2^-24 of magnitudes up to 10
+    assert float((x.grad.double() - want).abs().max()) <= 64 * 2.0 ** -24
+    with torch.no_grad():
+        again = class_logprobs_grad(x, None, class_logprobs(x, top=top), g_entropy=torch.ones(20, device="cuda"))
+    assert torch.equal(again, x.grad)
+
+
+def test_a_whole_step_captured_and_replayed():
+    """Lookup, log probabilities and both gradients in one graph, replayed on new ids and labels."""
+    from trspmm import class_logprobs, embedding
+    g = torch.Generator(device="cuda").manual_seed(0)
+    table = torch.randn(5000, 47, generator=g, device="cuda").half().requires_grad_()
+    ids = torch.randint(0, 5000, (6000,), generator=g, device="cuda")
+    labels = torch.randint(0, 47, (6000,), generator=g, device="cuda")
+
+    def step():
+        r = class_logprobs(embedding(table, ids, scale=0.5), labels, top=2)
+        return (r.logprobs, r.top_ids, *torch.autograd.grad(r.logprobs.sum() + r.entropy.sum(), table))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    ids.copy_(torch.randint(0, 50, (6000,), generator=g, device="cuda"))
+    labels.copy_(torch.randint(0, 47, (6000,), generator=g, device="cuda"))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(held, step()))

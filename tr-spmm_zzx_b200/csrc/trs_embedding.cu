@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(kLookupThreads, 8) k_lookup(const TI* __restri
 // Positions sorted by id
 // ----------------------------------------------------------------------------------------------
 // Stable, so that a row's positions ascend.  Positions without a row (padding, outside the table) get the key `rows` and come last.
-// The keys have bits(rows) bits, sorted by up to 11 at a time: two passes for tables of up to 4 M rows.  Pass: the counts of
+// The keys have bits(rows) bits, sorted by up to 11 (many ids: 8) at a time: two passes for tables of up to 4 M rows.  Pass: the counts of
 // each digit in each tile, their prefix sums over the tiles, then every key to its place.
 constexpr int kSortThreads = 512, kSortWarps = kSortThreads / 32, kSortItems = 8, kTile = kSortThreads * kSortItems, kMaxDigit = 11;
 
@@ -171,7 +171,8 @@ __global__ void __launch_bounds__(kSortThreads, 2) k_digit_scatter(const void* _
         unsigned same = __ballot_sync(0xffffffffu, in);
 #pragma unroll
         for (int b = 0; b < kMaxDigit; ++b) {
-            const unsigned vote = __ballot_sync(0xffffffffu, digit >> b & 1);   // (bits past the digit are 0 for all)
+            if (b >= digit_bits) break;
+            const unsigned vote = __ballot_sync(0xffffffffu, digit >> b & 1);
             same &= digit >> b & 1 ? vote : ~vote;
         }
         const int before = __popc(same & ((1u << lane) - 1));
@@ -562,6 +563,7 @@ int with_lookup(int pieces, Fn fn) {
     return fn(integral_constant<int, 16>(), integral_constant<int, 2>(), integral_constant<int, 3>());
 }
 
+constexpr long long kManyIds = 1 << 19;
 constexpr long long kMaxIds = (1ll << 31) - (1 << 16), kMaxRows = (1ll << 31) - 2;
 constexpr long long kMaxStride = (1ll << 31) - 1;
 constexpr int kMaxFeatures = 1 << 20;
@@ -575,7 +577,10 @@ GradPlan grad_plan(long long n, long long rows, int F) {
     GradPlan p;
     int bits = 1;
     while (bits < 32 && (rows >> bits)) ++bits;   // keys 0 .. rows
-    p.digits = (bits + kMaxDigit - 1) / kMaxDigit;
+    // Narrow digits cost a pass more and far less per pass (2^20 ids: two passes of 11 bits 67 us, three of 7 bits 55); the launches
+    // decide where ids are few.
+    const int widest = n >= kManyIds ? 8 : kMaxDigit;
+    p.digits = (bits + widest - 1) / widest;
     p.digit_bits = (bits + p.digits - 1) / p.digits;
     p.tiles = (int)ceil_div64(n, kTile);
     // spans: up to about a thousand of them, of 512 positions or more
