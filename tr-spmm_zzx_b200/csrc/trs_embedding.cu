@@ -234,40 +234,90 @@ __global__ void __launch_bounds__(kSortThreads, 2) k_digit_scatter(const void* _
     }
 }
 
-// Up to kFewIds ids: one CTA sorts (key, position) words in shared memory by a bitonic network, the other CTAs empty the segments.
-// (4 K ids of a 16 K row table by the digit passes: six launches, 25 us of them; this one 5 us.)
-constexpr int kFewIds = 4096, kFewThreads = 1024;
+// Up to a tile of ids: one CTA does all passes in shared memory, the other CTAs empty the segments.
+// (4 096 ids of a table of 16 384 rows: 11 us; one id more, six launches, 24 us and as much again on the host.  A bitonic network: 36 us.)
+constexpr int kFewIds = kTile, kFewDigit = 8, kFewBins = 1 << kFewDigit;
 
-__global__ void __launch_bounds__(kFewThreads) k_sort_few(const void* __restrict__ ids, int ids64, long long rows, long long padding, int n,
-                                                          int size, uint2* __restrict__ words_out, int2* __restrict__ segment, int* __restrict__ popular) {
-    const int threads = blockDim.x;   // up to half of `size`, the power of two from 64 on that holds n
+__global__ void __launch_bounds__(kSortThreads) k_sort_few(const void* __restrict__ ids, int ids64, long long rows, long long padding, int n,
+                                                           int bits, uint2* __restrict__ words_out, int2* __restrict__ segment,
+                                                           int* __restrict__ popular) {
     if (blockIdx.x) {
-        empty_segments(segment, popular, rows, (long long)(blockIdx.x - 1) * threads + threadIdx.x, (long long)(gridDim.x - 1) * threads);
+        empty_segments(segment, popular, rows, (long long)(blockIdx.x - 1) * kSortThreads + threadIdx.x, (long long)(gridDim.x - 1) * kSortThreads);
         return;
     }
-    __shared__ unsigned long long s_word[kFewIds];
-    for (int i = threadIdx.x; i < size; i += threads)
-        s_word[i] = i < n ? (unsigned long long)key_of(load_id(ids, ids64, i), rows, padding) << 32 | (unsigned)i : ~0ull;
-    __syncthreads();
-    for (int run = 2; run <= size; run *= 2) {
-        for (int o = run / 2; o; o /= 2) {
-            for (int i = threadIdx.x; i < size / 2; i += threads) {
-                const int lo = 2 * i - (i & (o - 1)), hi = lo + o;
-                const unsigned long long a = s_word[lo], b = s_word[hi];
-                if ((a > b) == ((lo & run) == 0)) {
-                    s_word[lo] = b;
-                    s_word[hi] = a;
-                }
+    __shared__ uint2 s_word[kFewIds];
+    __shared__ unsigned short s_rank[kSortWarps][kFewBins], s_start[kFewBins];
+    __shared__ int s_sum[kFewBins / 64];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int rounds = (n + kSortThreads - 1) / kSortThreads, first = warp * (rounds * 32) + lane;   // a warp has neighbouring words
+    uint2 word[kSortItems];
+    unsigned short rank[kSortItems];
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k) {
+        const int i = first + k * 32;
+        word[k] = make_uint2(0, 0);
+        if (k < rounds && i < n) word[k] = make_uint2(key_of(load_id(ids, ids64, i), rows, padding), i);
+    }
+    for (int shift = 0; shift < bits; shift += kFewDigit) {
+        for (int k = threadIdx.x; k < kSortWarps * kFewBins / 2; k += kSortThreads) ((unsigned*)s_rank)[k] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kSortItems; ++k) {
+            if (k >= rounds) break;
+            const bool in = first + k * 32 < n;
+            const unsigned digit = (word[k].x >> shift) & (kFewBins - 1);
+            unsigned same = __ballot_sync(0xffffffffu, in);
+#pragma unroll
+            for (int b = 0; b < kFewDigit; ++b) {
+                const unsigned vote = __ballot_sync(0xffffffffu, digit >> b & 1);
+                same &= digit >> b & 1 ? vote : ~vote;
             }
-            // 32 neighbouring pairs of a distance up to 32 are 64 words of their own
-            if (o > 32 || (o == 1 && run >= 64)) __syncthreads();
-            else __syncwarp();
+            const int before = __popc(same & ((1u << lane) - 1));
+            int r = 0;
+            if (in) r = s_rank[warp][digit] + before;
+            __syncwarp();
+            if (in && before == 0) s_rank[warp][digit] += (unsigned short)__popc(same);
+            __syncwarp();
+            rank[k] = (unsigned short)r;
         }
+        __syncthreads();
+        // a pair of digits a thread: counters become the words of the digit in the warps before; then places of the digits
+        unsigned sum = 0;
+        int here = 0, incl = 0;
+        if (threadIdx.x < kFewBins / 2) {
+#pragma unroll
+            for (int w = 0; w < kSortWarps; ++w) {
+                unsigned* c = (unsigned*)&s_rank[w][2 * threadIdx.x];
+                const unsigned x = *c;
+                *c = sum;
+                sum += x;
+            }
+            here = incl = (int)(sum & 0xffff) + (int)(sum >> 16);
+            for (int o = 1; o < 32; o *= 2) {
+                const int y = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += y;
+            }
+            if (lane == 31) s_sum[warp] = incl;
+        }
+        __syncthreads();
+        if (threadIdx.x < kFewBins / 2) {
+            int at = incl - here;
+            for (int w = 0; w < warp; ++w) at += s_sum[w];
+            s_start[2 * threadIdx.x] = (unsigned short)at;
+            s_start[2 * threadIdx.x + 1] = (unsigned short)(at + (sum & 0xffff));
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kSortItems; ++k) {
+            const unsigned digit = (word[k].x >> shift) & (kFewBins - 1);
+            if (k < rounds && first + k * 32 < n) s_word[s_start[digit] + s_rank[warp][digit] + rank[k]] = word[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kSortItems; ++k)
+            if (k < rounds && first + k * 32 < n) word[k] = s_word[first + k * 32];
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += threads) {
-        words_out[i] = make_uint2((unsigned)(s_word[i] >> 32), (unsigned)s_word[i]);
-    }
+    for (int i = threadIdx.x; i < n; i += kSortThreads) words_out[i] = s_word[i];
 }
 
 // ----------------------------------------------------------------------------------------------
@@ -569,7 +619,7 @@ constexpr long long kMaxStride = (1ll << 31) - 1;
 constexpr int kMaxFeatures = 1 << 20;
 
 struct GradPlan {
-    int digits = 0, digit_bits = 0, tiles = 0, span = 0, spans = 0;
+    int bits = 0, digits = 0, digit_bits = 0, tiles = 0, span = 0, spans = 0;
     size_t words[2] = {}, counts = 0, total = 0, segment = 0, block_sum = 0, span_sum = 0, popular = 0, bytes = 0;
 };
 
@@ -577,6 +627,7 @@ GradPlan grad_plan(long long n, long long rows, int F) {
     GradPlan p;
     int bits = 1;
     while (bits < 32 && (rows >> bits)) ++bits;   // keys 0 .. rows
+    p.bits = bits;
     // Narrow digits cost a pass more and far less per pass (2^20 ids: two passes of 11 bits 67 us, three of 7 bits 55); the launches
     // decide where ids are few.
     const int widest = n >= kManyIds ? 8 : kMaxDigit;
@@ -702,12 +753,9 @@ extern "C" int trs_embedding_grad(const void* grad, int grad_type, long long gra
         if (!ws || workspace_bytes < p.bytes || (uintptr_t)ws % 16) return TRS_E_WORKSPACE;
         if (n <= kFewIds) {
             p.digits = 1;   // (the result is where a first pass leaves it)
-            int size = 64;
-            while (size < n) size *= 2;
-            const int threads = size / 2 < kFewThreads ? size / 2 : kFewThreads;
-            const long long zero = ceil_div64(rows, 4 * threads);
-            rc = launch(k_sort_few, dim3(1 + (unsigned)(zero < 2 * 148 ? zero : 2 * 148)), threads, 0, st, ids, ids64, rows, padding_id, (int)n, size,
-                        (uint2*)(ws + p.words[0]), (int2*)(ws + p.segment), (int*)(ws + p.popular));
+            const long long zero = ceil_div64(rows, 4 * kSortThreads);
+            rc = launch(k_sort_few, dim3(1 + (unsigned)(zero < 2 * 148 ? zero : 2 * 148)), kSortThreads, 0, st, ids, ids64, rows, padding_id, (int)n,
+                        p.bits, (uint2*)(ws + p.words[0]), (int2*)(ws + p.segment), (int*)(ws + p.popular));
             if (rc) return rc;
         } else for (int pass = 0; pass < p.digits; ++pass) {
             rc = pass == 0 ? sort_pass<true>(ids, ids64, rows, padding_id, ws, p, (int)n, pass, st)

@@ -312,7 +312,7 @@ struct Running {
     }
 };
 template <class T, int THREADS, bool MASKED>
-__global__ void __launch_bounds__(THREADS, THREADS == 32 ? 24 : 1280 / THREADS) k_row(const Forward a, int parts) {
+__global__ void __launch_bounds__(THREADS, THREADS == 32 ? 24 : (MASKED ? 1024 : 1280) / THREADS) k_row(const Forward a, int parts) {
     constexpr int WARPS = THREADS / 32, VEC = Row<T>::VEC, TURN = kTurn, WORDS = VEC / 4 + 1;
     const long long r = blockIdx.x / parts;
     const int part = (int)(blockIdx.x - r * parts);
