@@ -426,3 +426,15 @@ def test_rows_without_a_distribution_are_nan_wherever_they_lie(C):
                 assert bool(torch.isnan(d).all())
             elif broken:
                 assert bool(torch.isnan(d[:, keep]).all()) and float(d[:, ~keep].float().abs().max()) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C", [5, 47, 200, 500, 1000, 5000])
+def test_fp32_scores_that_differ_in_their_last_bits(C):
+    """The order of alternatives goes by all bits of a score, whatever part of them a comparison starts with."""
+    from trspmm import class_logprobs
+    i = torch.arange(C, device="cuda")
+    x = torch.stack([1.0 + ((i * 7919) % 61).float() * 2.0 ** -23, 1.0 + (i % 61).float() * 2.0 ** -23, -1.0 - (i % 61).float() * 2.0 ** -23,
+                     torch.where(i % 2 == 0, 1.0, 1.0 + 2.0 ** -23), (i % 3).float() * 2.0 ** -126])
+    for top in (1, 4, 32):
+        Ref(x, None, top).check(class_logprobs(x, top=top))

@@ -617,33 +617,33 @@ __device__ __forceinline__ void short_top(const Forward& a, long long r, const R
         }
     }
     if constexpr (sizeof(T) == 4) {
-    if (!__any_sync(0xffffffffu, close)) return;
-    for (int k = 0; k < a.top; ++k) {
-        float m = s.m;
-        if (k) {
-            m = -INFINITY;
+        if (!__any_sync(0xffffffffu, close)) return;
+        for (int k = 0; k < a.top; ++k) {
+            float m = s.m;
+            if (k) {
+                m = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < PER; ++i)
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) m = fmaxf(m, v[i][q]);
+#pragma unroll
+                for (int o = G / 2; o; o /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            }
+            int at = 0x7fffffff;
+#pragma unroll
+            for (int i = PER; i-- > 0;)
+#pragma unroll
+                for (int q = VEC; q-- > 0;)
+                    if (v[i][q] == m) at = row.first(g + i * G) + q;
+#pragma unroll
+            for (int o = G / 2; o; o /= 2) at = min(at, __shfl_xor_sync(0xffffffffu, at, o));
 #pragma unroll
             for (int i = 0; i < PER; ++i)
 #pragma unroll
-                for (int q = 0; q < VEC; ++q) m = fmaxf(m, v[i][q]);
-#pragma unroll
-            for (int o = G / 2; o; o /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                for (int q = 0; q < VEC; ++q)
+                    if (row.first(g + i * G) + q == at) v[i][q] = -INFINITY;
+            if (k % G == g && r < a.n) write_top(a, r, k, m > -INFINITY, at, m, s.m, log_S);
         }
-        int at = 0x7fffffff;
-#pragma unroll
-        for (int i = PER; i-- > 0;)
-#pragma unroll
-            for (int q = VEC; q-- > 0;)
-                if (v[i][q] == m) at = row.first(g + i * G) + q;
-#pragma unroll
-        for (int o = G / 2; o; o /= 2) at = min(at, __shfl_xor_sync(0xffffffffu, at, o));
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-#pragma unroll
-            for (int q = 0; q < VEC; ++q)
-                if (row.first(g + i * G) + q == at) v[i][q] = -INFINITY;
-        if (k % G == g && r < a.n) write_top(a, r, k, m > -INFINITY, at, m, s.m, log_S);
-    }
     }
 }
 
