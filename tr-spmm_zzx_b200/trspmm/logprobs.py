@@ -80,6 +80,13 @@ def _forward(logits, targets, top, mask, scale, ignore_id) -> ClassLogprobs:
     return ClassLogprobs(logprobs, entropy, top_logprobs, top_ids, stats)
 
 
+def _launch_grad(index, front, back, ignore_id, top_ids, stats, entropy, g_logprobs, g_entropy, g_top, dx, dx_stride):
+    _lib.launch(index, _lib.load().trs_logprobs_grad, *front, _NO_IGNORE if ignore_id is None else ignore_id, *back,
+                None if g_top is None else top_ids.data_ptr(), stats.data_ptr(), None if g_entropy is None else entropy.data_ptr(),
+                None if g_logprobs is None else g_logprobs.data_ptr(), None if g_entropy is None else g_entropy.data_ptr(),
+                None if g_top is None else g_top.data_ptr(), dx.data_ptr(), dx_stride)
+
+
 class _LogprobsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top, mask, scale, ignore_id):
@@ -98,9 +105,11 @@ class _LogprobsFn(torch.autograd.Function):
         scale, ignore_id = ctx.args
         if g_logprobs is None and g_entropy is None and g_top is None:
             return (None,) * 6
-        dx = class_logprobs_grad(logits, targets, ClassLogprobs(None, entropy, None, top_ids, stats),
-                                 *[None if g is None else g.contiguous() for g in (g_logprobs, g_entropy, g_top)],
-                                 mask=mask, scale=scale, ignore_id=ignore_id)
+        top = 0 if g_top is None else g_top.shape[-1]
+        index, front, back = _check(logits, targets, mask, scale, top)
+        dx = torch.empty_like(logits, memory_format=torch.contiguous_format)
+        _launch_grad(index, front, back, ignore_id, top_ids, stats, entropy, *[None if g is None else g.contiguous() for g in
+                                                                              (g_logprobs, g_entropy, g_top)], dx, logits.shape[1])
         return dx, None, None, None, None, None
 
     once = torch.autograd.function.once_differentiable(lambda ctx, *g: _LogprobsFn.backward(ctx, *g))
@@ -153,9 +162,6 @@ def class_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor | None, resu
     else:
         dx_stride = _row_stride(out, "out")
 
-    def ptr(t):
-        return None if t is None else t.data_ptr()
-    _lib.launch(index, _lib.load().trs_logprobs_grad, *front, _NO_IGNORE if ignore_id is None else ignore_id, *back,
-                ptr(result.top_ids) if top else None, result.stats.data_ptr(), ptr(result.entropy) if g_entropy is not None else None,
-                ptr(g_logprobs), ptr(g_entropy), ptr(g_top_logprobs) if top else None, out.data_ptr(), dx_stride)
+    _launch_grad(index, front, back, ignore_id, result.top_ids, result.stats, result.entropy, g_logprobs, g_entropy,
+                 g_top_logprobs if top else None, out, dx_stride)
     return out
