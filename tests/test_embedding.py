@@ -239,6 +239,27 @@ def test_grad_popular_rows(pattern, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("gap", [1, 3, 1000])
+@pytest.mark.parametrize("F,dtype", [(40, F16), (3, F32), (300, BF16)])
+def test_grad_rows_of_every_length_side_by_side(gap, F, dtype):
+    """Rows of a few positions, of as many as make a row popular, of blocks and spans, next to each other and apart."""
+    from trspmm import embedding_grad
+    lengths = torch.tensor([0, 1, 2, 7, 8, 9, 22, 23, 24, 25, 26, 47, 63, 64, 65, 0, 127, 128, 129, 24, 24, 500, 511, 512, 513, 1, 1025, 23] * 3,
+                           device="cuda")
+    ids = torch.repeat_interleave(torch.arange(lengths.numel(), device="cuda") * gap, lengths)
+    rows = lengths.numel() * gap + 5
+    for order in (torch.arange(ids.numel(), device="cuda"), torch.randperm(ids.numel(), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")):
+        g = _randn(ids.numel(), F, dtype=dtype, seed=7)
+        got = embedding_grad(g, ids[order], rows, out_dtype=F32)
+        ref, extra = _grad_ref(g, ids[order], rows, 1.0)
+        _within(got, ref, extra, F32)
+        out = torch.ones(rows, F, device="cuda")
+        embedding_grad(g, ids[order], rows, out=out, accumulate=True)
+        _within(out, ref + 1.0, extra + 4 * U, F32)
+        assert bool((out[got.abs().sum(1) == 0] == 1).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("idt", [torch.int32, torch.int64])
 def test_grad_padding_ids_outside_and_nothing_left(idt):
     from trspmm import embedding_grad

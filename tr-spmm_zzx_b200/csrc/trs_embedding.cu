@@ -325,9 +325,11 @@ __global__ void __launch_bounds__(kSortThreads) k_sort_few(const void* __restric
 // ----------------------------------------------------------------------------------------------
 // The sorted positions are cut into blocks of 64 and spans of several blocks.  A block whose positions all name one row is summed
 // ahead (a span of one row as a whole), all of them in parallel, so that a row with a hundred thousand positions is not one
-// group's work.  Rows with such blocks are noted in a list (popular[0] of them, in any order) and get a CTA each, the
-// first ones of k_sums: as part of their neighbours' work they were its last 60 us where others were done.
-constexpr int kBlock = 64, kSpanWarps = kThreads / 32;
+// group's work.  Rows with kPopular positions or more are noted in a list (popular[0] of them, in any order) and get a CTA each, the
+// first ones of k_sums: as part of their neighbours' work a hub was its last 60 us where others were done, and a table whose rows are in
+// the order of their popularity took 336 us where the same ids spread over it took 196 (now 197; from 16 positions on 184, but 600 k ids of
+// 50 k rows 99 us for 74).
+constexpr int kBlock = 64, kSpanWarps = kThreads / 32, kPopular = 24;
 
 template <class T, int VEC>
 __device__ __forceinline__ void add_row(float (&acc)[VEC], const T* __restrict__ row, int c) {
@@ -381,6 +383,8 @@ __global__ void __launch_bounds__(kThreads, 4) k_block_sums(const T* __restrict_
                        k1_down = __shfl_down_sync(none, k1, 1), k0_last = __shfl_sync(none, k0, 31), k1_first = __shfl_sync(none, k1, 0);
         auto note = [&](int i, unsigned k, unsigned before, unsigned after) {
             if (k >= rows) return;
+            if (before != k && after == k && i < n - (kPopular - 1) && words[i + kPopular - 1].x == k)
+                popular[1 + atomicAdd(popular, 1)] = (int)k;
             if (before != k && after != k) segment[k] = make_int2(i, i + 1);
             else if (before != k) segment[k].x = i;
             else if (after != k) segment[k].y = i + 1;
@@ -389,7 +393,6 @@ __global__ void __launch_bounds__(kThreads, 4) k_block_sums(const T* __restrict_
         note(i1, k1, lane ? k1_up : k0_last, lane < 31 ? k1_down : edge);
         const unsigned key = __shfl_sync(none, k0, 0);
         if (!__all_sync(none, k0 == key && k1 == key) || key >= rows) continue;   // (the end of the list is not: none)
-        if (lane == 0 && (b == 0 || words[b - kBlock].x != key)) popular[1 + atomicAdd(popular, 1)] = (int)key;   // its first block
         if (whole) continue;
         const int pa = (int)w0.y, pb = (int)w1.y;
         for (int c0 = 0; c0 < pieces; c0 += G) {
@@ -427,12 +430,11 @@ __global__ void __launch_bounds__(kThreads, 4) k_block_sums(const T* __restrict_
     }
 }
 
-// A group of G lanes writes kSumRows neighbouring rows, G pieces of each.  Their positions are neighbours too: where none of the rows is
+// A group of G lanes writes ROWS neighbouring rows, G pieces of each.  Their positions are neighbours too: where none of the rows is
 // popular, the group streams through them, kSumBatch at a time, and writes a row when the key changes; otherwise it goes row by row.
-constexpr int kSumThreads = 128, kSumRows = 8, kSumBatch = 4;
+constexpr int kSumThreads = 128, kSumBatch = 4;
 
-__device__ __forceinline__ int block_up(int p) { return (p + kBlock - 1) & ~(kBlock - 1); }
-__device__ __forceinline__ bool is_popular(int2 s) { return block_up(s.x) + kBlock <= s.y; }   // holds a block
+__device__ __forceinline__ bool is_popular(int2 s) { return s.y - s.x >= kPopular; }
 
 template <class TO, int VEC>
 __device__ __forceinline__ void write_sum(TO* __restrict__ o, const float (&acc)[VEC], float scale, int accumulate) {
@@ -469,7 +471,8 @@ __device__ __forceinline__ void sum_popular(const SumArgs<TI, TO>& a, long long 
     constexpr int GROUPS = kSumThreads / G;
     const int group = threadIdx.x / G, lane = threadIdx.x % G, pieces = a.F / VEC;
     const int2 s = a.segment[v];
-    const int b0 = block_up(s.x), b1 = s.y & ~(kBlock - 1);                               // whole blocks
+    int b0 = (s.x + kBlock - 1) & ~(kBlock - 1), b1 = s.y & ~(kBlock - 1);                // whole blocks
+    if (b0 > b1) b0 = b1 = s.y;
     const int t0 = (int)min(((long long)b0 + a.span - 1) / a.span * a.span, (long long)b1), t1 = max(b1 / a.span * a.span, t0);   // whole spans
     const int head = b0 - s.x, singles = head + s.y - b1;
     const int before = (t0 - b0) / kBlock, spans = (t1 - t0) / a.span, parts = before + spans + (b1 - t1) / kBlock;
@@ -504,7 +507,7 @@ __device__ __forceinline__ void sum_popular(const SumArgs<TI, TO>& a, long long 
     }
 }
 
-template <class TI, class TO, int VEC, int G>
+template <class TI, class TO, int VEC, int G, int ROWS>
 __global__ void __launch_bounds__(kSumThreads) k_sums(const SumArgs<TI, TO> a) {
     __shared__ float s_part[kSumThreads / G][G * VEC];
     wait_for_kernel_before();
@@ -513,7 +516,7 @@ __global__ void __launch_bounds__(kSumThreads) k_sums(const SumArgs<TI, TO> a) {
         return;
     }
     const long long item = ((long long)(blockIdx.x - a.popular_ctas) * kSumThreads + threadIdx.x) / G;
-    const long long set = a.slabs == 1 ? item : item / a.slabs, v0 = set * kSumRows;
+    const long long set = a.slabs == 1 ? item : item / a.slabs, v0 = set * ROWS;
     const int c = (a.slabs == 1 ? 0 : (int)(item - set * a.slabs) * G) + threadIdx.x % G;
     if (v0 >= a.rows || c >= a.F / VEC) return;
     const TI* __restrict__ g = a.g + (size_t)c * VEC;
@@ -521,11 +524,11 @@ __global__ void __launch_bounds__(kSumThreads) k_sums(const SumArgs<TI, TO> a) {
     int begin = a.n, end_all = 0;
     bool popular = false;
     {
-        int2 s[kSumRows];
+        int2 s[ROWS];
 #pragma unroll
-        for (int u = 0; u < kSumRows; ++u) s[u] = a.n > 0 ? a.segment[min(v0 + u, a.rows - 1)] : make_int2(0, 0);
+        for (int u = 0; u < ROWS; ++u) s[u] = a.n > 0 ? a.segment[min(v0 + u, a.rows - 1)] : make_int2(0, 0);
 #pragma unroll
-        for (int u = 0; u < kSumRows; ++u) {
+        for (int u = 0; u < ROWS; ++u) {
             if (s[u].x < s[u].y && v0 + u < a.rows) {
                 begin = min(begin, s[u].x);
                 end_all = max(end_all, s[u].y);
@@ -559,7 +562,7 @@ __global__ void __launch_bounds__(kSumThreads) k_sums(const SumArgs<TI, TO> a) {
             }
         }
     };
-    const int runs = popular ? kSumRows : 1;
+    const int runs = popular ? ROWS : 1;
     for (int u = 0; u < runs; ++u) {
         int2 s = make_int2(begin, end_all);
         if (popular) {
@@ -650,7 +653,7 @@ GradPlan grad_plan(long long n, long long rows, int F) {
     p.segment = take((size_t)(rows + 1) * 8);
     p.block_sum = take((size_t)(n / kBlock) * F * 4);
     p.span_sum = take((size_t)p.spans * F * 4);
-    p.popular = take((size_t)(n / kBlock + 1) * 4);
+    p.popular = take((size_t)(n / kPopular + 1) * 4);
     p.bytes = at;
     return p;
 }
@@ -789,13 +792,17 @@ extern "C" int trs_embedding_grad(const void* grad, int grad_type, long long gra
                             return (int)TRS_E_ARG;   // not reached: elements_per_piece
                         } else {
                             const int slabs = ceil_div(pieces, G);
-                            const long long threads = ceil_div64(rows, kSumRows) * slabs * G;
-                            if (ceil_div64(threads, kSumThreads) > 0x7fff0000ll) return (int)TRS_E_LIMIT;
-                            const int popular_ctas = (int)(n / kBlock < 2 * 148 ? n / kBlock : 2 * 148);
+                            const int popular_ctas = (int)(n / kPopular < 8 * 148 ? n / kPopular : 8 * 148);
                             const SumArgs<TI, TO> args{(const TI*)grad, grad_stride, words, (int)n, rows, F, slabs, p.span, segment, block_sum, span_sum,
                                                        popular, popular_ctas, scale, (TO*)out, out_stride, accumulate};
-                            return launch_behind(k_sums<TI, TO, VEC, G>, dim3((unsigned)(popular_ctas + ceil_div64(threads, kSumThreads))),
-                                                 kSumThreads, 0, st, n > 0, args);
+                            auto run = [&](auto rows_a_group) {
+                                constexpr int ROWS = decltype(rows_a_group)::value;
+                                const long long ctas = ceil_div64(ceil_div64(rows, ROWS) * slabs * G, kSumThreads);
+                                if (ctas > 0x7fff0000ll) return (int)TRS_E_LIMIT;
+                                return launch_behind(k_sums<TI, TO, VEC, G, ROWS>, dim3((unsigned)(popular_ctas + ctas)), kSumThreads, 0, st, n > 0, args);
+                            };
+                            // eight rows where most have no more than a position or two, otherwise their positions are a long chain
+                            return n > 2 * rows ? run(std::integral_constant<int, 2>()) : run(std::integral_constant<int, 8>());
                         }
                     });
                 });
