@@ -438,3 +438,36 @@ def test_fp32_scores_that_differ_in_their_last_bits(C):
                      torch.where(i % 2 == 0, 1.0, 1.0 + 2.0 ** -23), (i % 3).float() * 2.0 ** -126])
     for top in (1, 4, 32):
         Ref(x, None, top).check(class_logprobs(x, top=top))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("C", [4, 7, 47, 255, 600, 1025, 5000, 66000])
+@pytest.mark.parametrize("layout", ["plain", "apart", "masked"])
+def test_weights_of_a_row_that_cancel(C, dtype, layout):
+    """Margins: the weights of a row's target and alternatives add up to 0 (small whole numbers: exactly), and are not 0."""
+    from trspmm import class_logprobs, class_logprobs_grad
+    n = 30
+    x = _scores(n, C, dtype, width=C + 3 if layout == "apart" else None, offset=1 if layout == "apart" else 0)
+    g = torch.Generator(device="cuda").manual_seed(C)
+    mask = None
+    if layout == "masked":
+        mask = torch.rand(n, C, generator=g, device="cuda") < 0.7
+        mask[7], mask[8] = False, False
+        mask[8, C - 1] = True
+        x = torch.where(mask, x, float("nan"))
+    targets = torch.randint(0, C, (n,), generator=g, device="cuda")
+    best = Ref(x, targets, 2, mask).top_ids.long()
+    targets[10:15], targets[15:20] = best[10:15, 0].clamp(min=0), best[15:20, 1].clamp(min=0)   # the target is an alternative too
+    kinds = torch.tensor([[0, 1, -1, 0], [1, -1, 0, 0], [2, -1, -1, 0], [-3, 1, 1, 1], [1, 0, 0, -1]], dtype=F32, device="cuda")
+    w = kinds.repeat(n // 5, 1)
+    w[29] = 0
+    g_lp, g_top = w[:, 0].contiguous(), w[:, 1:].contiguous()
+    some = torch.where(torch.arange(n, device="cuda") % 3 == 0, 0.5, 0.0)
+    for g_h in (None, some):
+        leaf = x.detach().requires_grad_()
+        r = class_logprobs(leaf, targets, top=3, mask=mask, scale=1.25)
+        outs = (r.logprobs, r.top_logprobs) if g_h is None else (r.logprobs, r.top_logprobs, r.entropy)
+        grad, = torch.autograd.grad(outs, leaf, (g_lp, g_top) if g_h is None else (g_lp, g_top, g_h))
+        Ref(x, targets, 3, mask, 1.25).check(r, grad, (g_lp, g_h, g_top))
+        assert torch.equal(grad, class_logprobs_grad(x, targets, r, g_lp, g_h, g_top, mask, 1.25))
