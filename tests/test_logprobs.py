@@ -471,3 +471,28 @@ def test_weights_of_a_row_that_cancel(C, dtype, layout):
         grad, = torch.autograd.grad(outs, leaf, (g_lp, g_top) if g_h is None else (g_lp, g_top, g_h))
         Ref(x, targets, 3, mask, 1.25).check(r, grad, (g_lp, g_h, g_top))
         assert torch.equal(grad, class_logprobs_grad(x, targets, r, g_lp, g_h, g_top, mask, 1.25))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("C", [6, 47, 600, 5000, 66000])
+def test_alternatives_alone_of_rows_without_a_distribution(C, dtype):
+    """Where the forward call gave NaN, so does the gradient of its alternatives - in every place that is not masked, and unless all
+    weights are 0."""
+    from trspmm import class_logprobs
+    x = _scores(7, C, dtype)
+    x[1, C - 1], x[2, 0], x[3, C // 2], x[4, 3], x[5, 2] = float("nan"), float("inf"), float("nan"), float("inf"), float("nan")
+    keep = torch.ones(7, C, dtype=torch.bool, device="cuda")
+    keep[:, 1] = False
+    keep[5, 2] = False   # its NaN is masked
+    keep[6] = False
+    w = torch.tensor([[1, 2], [1, 2], [1, -1], [0, 3], [0, 0], [1, 2], [1, 2]], dtype=F32, device="cuda")
+    for mask in (None, keep):
+        broken = [1, 2, 3] + ([5] if mask is None else [])
+        leaf = x.clone().requires_grad_()
+        r = class_logprobs(leaf, top=2, mask=mask)
+        d, = torch.autograd.grad(r.top_logprobs, leaf, w)
+        for k in range(7):
+            may = torch.ones_like(keep[k]) if mask is None else mask[k]
+            assert bool((torch.isnan(d[k]) == (may & (k in broken))).all()), (k, mask is None)
+            assert k in broken or k in (0, 5) or (k == 6 and mask is None) or float(d[k].float().abs().max()) == 0

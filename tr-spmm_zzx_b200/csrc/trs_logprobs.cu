@@ -738,12 +738,14 @@ __device__ __forceinline__ RowGrad row_grad(const Backward& a, long long r) {
     float A = 0.f;
     if (a.g_logprobs && target_counts(a, load_target(a.target, a.target64, r))) A = a.g_logprobs[r];
     bool weights = A != 0.f;   // any: their sum may be 0 where they are not (a margin of two classes)
+    const bool broken = !(st.x < INFINITY);   // no alternatives there, and NaN for their log probabilities
     if (a.g_top)
         for (int k = 0; k < a.top; ++k) {
-            if (a.top_ids[r * a.top + k] < 0) continue;
+            const bool has = a.top_ids[r * a.top + k] >= 0;
+            if (!has && !broken) continue;
             const float t = a.g_top[r * a.top + k];
             weights |= t != 0.f;
-            A += t;
+            if (has) A += t;
         }
     const float b = a.g_entropy ? a.g_entropy[r] : 0.f;
     RowGrad g;
@@ -751,7 +753,7 @@ __device__ __forceinline__ RowGrad row_grad(const Backward& a, long long r) {
     g.c = a.c;
     g.zero = st.x == -INFINITY || (!weights && b == 0.f);
     // log p + entropy = d ln 2 - log S + entropy
-    g.inv_S = st.x < INFINITY ? 1.f / st.y : NAN;
+    g.inv_S = broken ? NAN : 1.f / st.y;
     g.A = b == 0.f ? A : A + b * (a.entropy[r] - logf(st.y));
     g.B = b * kLn2;
     return g;
