@@ -392,3 +392,29 @@ def test_calls_from_several_threads():
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not wrong
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("table,out", [(F16, F16), (F32, F16), (BF16, F32)])
+def test_forward_mode_is_refused(table, out):
+    """A tangent is not dropped in silence, whichever operand has it."""
+    import torch.autograd.forward_ad as fw
+    from trspmm import embedding, embedding_grad
+    W, ids, g = _randn(8, 16, dtype=table), _ids(6, 8), _randn(6, 16, dtype=table)
+    plain = embedding(W, ids, out_dtype=out)
+    with fw.dual_level():
+        dual, dual_g = fw.make_dual(W, torch.ones_like(W)), fw.make_dual(g, torch.ones_like(g))
+        dual_out = fw.make_dual(torch.zeros_like(plain), torch.ones_like(plain))
+        for call in (lambda: embedding(dual, ids, out_dtype=out), lambda: embedding(dual, ids, out=torch.empty_like(plain)),
+                     lambda: embedding(W, ids, out=dual_out), lambda: embedding_grad(dual_g, ids, 8),
+                     lambda: embedding_grad(dual_g, ids, 8, out=torch.empty_like(W)), lambda: embedding_grad(g, ids, 8, out=dual)):
+            with pytest.raises(RuntimeError):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError):
+                call()
+        leaf = W.clone().requires_grad_()
+        y = embedding(leaf, ids)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y, leaf, dual_g)
+        assert torch.equal(embedding(W, ids, out_dtype=out), plain)   # no tangent: as outside the level
+    assert torch.equal(embedding(W, ids, out_dtype=out), plain)

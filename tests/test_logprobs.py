@@ -496,3 +496,31 @@ def test_alternatives_alone_of_rows_without_a_distribution(C, dtype):
             may = torch.ones_like(keep[k]) if mask is None else mask[k]
             assert bool((torch.isnan(d[k]) == (may & (k in broken))).all()), (k, mask is None)
             assert k in broken or k in (0, 5) or (k == 6 and mask is None) or float(d[k].float().abs().max()) == 0
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused():
+    """A tangent is not dropped in silence, whichever operand has it."""
+    import torch.autograd.forward_ad as fw
+    from trspmm import class_logprobs, class_logprobs_grad
+    x, t, one = _scores(4, 10, F32), torch.zeros(4, dtype=torch.int64, device="cuda"), torch.ones(4, device="cuda")
+    r = class_logprobs(x, t, top=2)
+    two = torch.ones(4, 2, device="cuda")
+    with fw.dual_level():
+        def dual(v):
+            return fw.make_dual(v.clone(), torch.ones_like(v))
+        for call in (lambda: class_logprobs(dual(x), t), lambda: class_logprobs(dual(x), top=1),
+                     lambda: class_logprobs_grad(dual(x), t, r, one), lambda: class_logprobs_grad(x, t, r, dual(one)),
+                     lambda: class_logprobs_grad(x, t, r, g_entropy=dual(one)), lambda: class_logprobs_grad(x, t, r, g_top_logprobs=dual(two)),
+                     lambda: class_logprobs_grad(x, t, r._replace(stats=dual(r.stats)), one),
+                     lambda: class_logprobs_grad(x, t, r._replace(entropy=dual(r.entropy)), g_entropy=one),
+                     lambda: class_logprobs_grad(x, t, r, one, out=dual(x))):
+            with pytest.raises(RuntimeError):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError):
+                call()
+        leaf = x.clone().requires_grad_()
+        y = class_logprobs(leaf, t)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y.logprobs, leaf, dual(one))
+        assert torch.equal(class_logprobs(x, t).logprobs, r.logprobs)

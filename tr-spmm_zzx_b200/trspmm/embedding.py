@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -51,6 +52,13 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
         return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
     (a0, a1), (b0, b1) = span(a), span(b)
     return a0 < b1 and b0 < a1
+
+
+def _no_tangents(what: str, *tensors) -> None:
+    """Refuses tensors with a tangent: there is no forward-mode derivative, and the kernels would drop it in silence.  (Outside a
+    level of forward_ad, where there are none, this is one comparison.)"""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 def _lookup(table, ids, scale, padding_id, dtype, out):
@@ -109,7 +117,8 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, paddin
     `padding_id` gives zeros, one outside [0, rows) a row of NaN.  out_dtype: the table's type unless given - an fp32 table gives
     the fp16 features that the SpMM takes without a copy of the table.  `out` may be given instead (for a vector of ids its rows
     may lie apart).  Differentiable in the table where no `out` is given: the gradient is embedding_grad's, dense, in the
-    table's type."""
+    table's type.  Forward-mode differentiation is refused."""
+    _no_tangents("embedding", table, out)
     if table.requires_grad and torch.is_grad_enabled():
         if out is not None:
             raise ValueError("embedding with out= is not differentiable: call it under torch.no_grad()")
@@ -127,6 +136,7 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: fl
     once to out_dtype (the type of `grad` unless given).  Rows that no id names are zero.  With `accumulate` the sums
     are added to `out`, whose other rows stay as they are (micro-batches).  Padding ids and ids outside the table contribute
     nothing."""
+    _no_tangents("embedding_grad", grad, out)
     index = grad.get_device()
     if index < 0:
         raise ValueError("embedding_grad needs CUDA tensors (there is no CPU fallback)")

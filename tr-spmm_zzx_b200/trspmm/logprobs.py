@@ -12,7 +12,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .embedding import _overlap, _row_stride, _type_code
+from .embedding import _no_tangents, _overlap, _row_stride, _type_code
 
 MAX_TOP = 32
 _NO_IGNORE = -(1 << 63)
@@ -101,6 +101,7 @@ class _LogprobsFn(torch.autograd.Function):
     def backward(ctx, g_logprobs, g_entropy, g_top, _ids, _stats):
         if torch.is_grad_enabled():   # under create_graph
             return _LogprobsFn.once(ctx, g_logprobs, g_entropy, g_top, _ids, _stats)
+        _no_tangents("the gradient of class_logprobs", g_logprobs, g_entropy, g_top)
         logits, targets, mask, entropy, top_ids, stats = ctx.saved_tensors
         scale, ignore_id = ctx.args
         if g_logprobs is None and g_entropy is None and g_top is None:
@@ -125,7 +126,9 @@ def class_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
     -inf, entropy 0 and alternatives -1.  Alternatives (up to 32) descend by score, the lowest class first among equal ones.
     Computed in fp32, results are fp32 (top_ids int32).
 
-    Differentiable in the logits through logprobs, entropy and top_logprobs (not through the choice of the alternatives)."""
+    Differentiable in the logits through logprobs, entropy and top_logprobs (not through the choice of the alternatives).  Forward-mode
+    differentiation is refused."""
+    _no_tangents("class_logprobs", logits)
     if logits.requires_grad and torch.is_grad_enabled():
         return ClassLogprobs(*_LogprobsFn.apply(logits, targets, top, mask, scale, ignore_id))
     return _forward(logits, targets, top, mask, scale, ignore_id)
@@ -138,6 +141,7 @@ def class_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor | None, resu
     """The gradient of the logits, of their shape and type, from the gradients (fp32, contiguous) of what class_logprobs
     returned for the same arguments as `result` (its entropy is read where g_entropy is given, its top_ids where g_top_logprobs
     is, its stats always)."""
+    _no_tangents("class_logprobs_grad", logits, result.stats, result.entropy, g_logprobs, g_entropy, g_top_logprobs, out)
     top = 0 if g_top_logprobs is None else g_top_logprobs.shape[-1]
     index, front, back = _check(logits, targets, mask, scale, top)
     n = logits.shape[0]
