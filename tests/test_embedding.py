@@ -418,3 +418,28 @@ def test_forward_mode_is_refused(table, out):
             torch.autograd.grad(y, leaf, dual_g)
         assert torch.equal(embedding(W, ids, out_dtype=out), plain)   # no tangent: as outside the level
     assert torch.equal(embedding(W, ids, out_dtype=out), plain)
+
+
+@pytest.mark.gpu
+def test_results_written_in_place_are_noticed_by_autograd():
+    """out= changes a tensor that a graph may have kept: its backward pass raises as after any change in place."""
+    from trspmm import embedding, embedding_grad
+    W, ids = _randn(8, 16), _ids(6, 8)
+    for write in (lambda t: embedding(W, ids, out=t), lambda t: embedding(W, ids, out=t[:, :]),
+                  lambda t: embedding_grad(_randn(9, 16), _ids(9, 6), 6, out=t),
+                  lambda t: embedding_grad(_randn(9, 16), _ids(9, 6), 6, out=t, accumulate=True)):
+        w = torch.ones(6, 16, device="cuda", requires_grad=True)
+        kept = torch.ones(6, 16, device="cuda")
+        y = w * kept
+        write(kept)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    leaf = torch.ones(6, 16, device="cuda", requires_grad=True)
+    for out in (leaf, leaf * 2):   # what autograd follows is not overwritten behind its back
+        for call in (lambda: embedding(W, ids, out=out), lambda: embedding_grad(_randn(9, 16), _ids(9, 6), 6, out=out)):
+            with pytest.raises(ValueError):
+                call()
+            with torch.no_grad():
+                assert call() is out
+    with torch.inference_mode():
+        assert torch.equal(embedding(W, ids, out=torch.empty(6, 16, device="cuda")), W[ids])

@@ -524,3 +524,18 @@ def test_forward_mode_is_refused():
         with pytest.raises(RuntimeError):
             torch.autograd.grad(y.logprobs, leaf, dual(one))
         assert torch.equal(class_logprobs(x, t).logprobs, r.logprobs)
+
+
+@pytest.mark.gpu
+def test_a_gradient_written_in_place_is_noticed_by_autograd():
+    """out= changes a tensor that a graph may have kept: its backward pass raises as after any change in place."""
+    from trspmm import class_logprobs, class_logprobs_grad
+    x, t = _scores(4, 10, F32), torch.zeros(4, dtype=torch.int64, device="cuda")
+    w = torch.ones(4, 10, device="cuda", requires_grad=True)
+    kept = torch.ones(4, 10, device="cuda")
+    y = w * kept
+    class_logprobs_grad(x, t, class_logprobs(x, t), torch.ones(4, device="cuda"), out=kept)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with pytest.raises(ValueError):
+        class_logprobs_grad(x, t, class_logprobs(x, t), torch.ones(4, device="cuda"), out=w)

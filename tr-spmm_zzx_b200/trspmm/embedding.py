@@ -61,6 +61,16 @@ def _no_tangents(what: str, *tensors) -> None:
         raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
+def _written(out: torch.Tensor) -> None:
+    """Tells autograd that the kernels write the caller's tensor: a graph that kept it raises in its backward pass."""
+    torch.autograd.graph.increment_version(out)
+
+
+def _check_out(what: str, out) -> None:
+    if out is not None and out.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what} with out= is not differentiable: call it under torch.no_grad()")
+
+
 def _lookup(table, ids, scale, padding_id, dtype, out):
     index = table.get_device()
     if index < 0:
@@ -87,6 +97,7 @@ def _lookup(table, ids, scale, padding_id, dtype, out):
             raise ValueError("out must be contiguous unless ids is a vector")
         if _overlap(out, table) or _overlap(out, ids):
             raise ValueError("out may not overlap the table or the ids")
+        _written(out)
     _lib.launch(index, _lib.load().trs_embedding, table.data_ptr(), code, rows, stride, ids.data_ptr(), wide, ids.numel(), F, scale,
                 _NO_PADDING if padding_id is None else padding_id, out.data_ptr(), out_code, out_stride)
     return out
@@ -119,6 +130,7 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, paddin
     may lie apart).  Differentiable in the table where no `out` is given: the gradient is embedding_grad's, dense, in the
     table's type.  Forward-mode differentiation is refused."""
     _no_tangents("embedding", table, out)
+    _check_out("embedding", out)
     if table.requires_grad and torch.is_grad_enabled():
         if out is not None:
             raise ValueError("embedding with out= is not differentiable: call it under torch.no_grad()")
@@ -137,6 +149,7 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: fl
     are added to `out`, whose other rows stay as they are (micro-batches).  Padding ids and ids outside the table contribute
     nothing."""
     _no_tangents("embedding_grad", grad, out)
+    _check_out("embedding_grad", out)
     index = grad.get_device()
     if index < 0:
         raise ValueError("embedding_grad needs CUDA tensors (there is no CPU fallback)")
@@ -164,6 +177,7 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: fl
         if _overlap(out, grad) or _overlap(out, ids):
             raise ValueError("out may not overlap the gradient or the ids")
         out_code, out_stride = _type_code(out.dtype, "the output"), _row_stride(out, "out")
+        _written(out)
     lib, need = _lib.load(), C.c_size_t()
     _lib.check(lib.trs_embedding_grad_workspace_bytes(n, n_rows, F, C.byref(need)))
     # the workspace is this call's own: calls on several streams, and graphs, do not share one

@@ -12,7 +12,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .embedding import _no_tangents, _overlap, _row_stride, _type_code
+from .embedding import _check_out, _no_tangents, _overlap, _row_stride, _type_code, _written
 
 MAX_TOP = 32
 _NO_IGNORE = -(1 << 63)
@@ -142,6 +142,7 @@ def class_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor | None, resu
     returned for the same arguments as `result` (its entropy is read where g_entropy is given, its top_ids where g_top_logprobs
     is, its stats always)."""
     _no_tangents("class_logprobs_grad", logits, result.stats, result.entropy, g_logprobs, g_entropy, g_top_logprobs, out)
+    _check_out("class_logprobs_grad", out)
     top = 0 if g_top_logprobs is None else g_top_logprobs.shape[-1]
     index, front, back = _check(logits, targets, mask, scale, top)
     n = logits.shape[0]
@@ -165,6 +166,7 @@ def class_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor | None, resu
         raise ValueError("out may not overlap the logits")
     else:
         dx_stride = _row_stride(out, "out")
+        _written(out)
 
     _launch_grad(index, front, back, ignore_id, result.top_ids, result.stats, result.entropy, g_logprobs, g_entropy,
                  g_top_logprobs if top else None, out, dx_stride)
