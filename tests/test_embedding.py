@@ -443,3 +443,16 @@ def test_results_written_in_place_are_noticed_by_autograd():
                 assert call() is out
     with torch.inference_mode():
         assert torch.equal(embedding(W, ids, out=torch.empty(6, 16, device="cuda")), W[ids])
+
+
+@pytest.mark.gpu
+def test_ids_that_64_bits_do_not_hold_are_refused():
+    """They do not come back as other ids."""
+    from trspmm import embedding, embedding_grad
+    W, ids = _randn(8, 16, dtype=F16), _ids(6, 8)
+    for bad in (1 << 64, (1 << 64) + 3, 1 << 63, -(1 << 63), -(1 << 64) + 1):
+        for call in (lambda: embedding(W, ids, padding_id=bad), lambda: embedding_grad(W[:6], ids, 8, padding_id=bad)):
+            with pytest.raises(ValueError):
+                call()
+    for far in ((1 << 63) - 1, 1 - (1 << 63)):
+        assert torch.equal(embedding(W, ids, padding_id=far), W[ids])

@@ -539,3 +539,17 @@ def test_a_gradient_written_in_place_is_noticed_by_autograd():
         y.sum().backward()
     with pytest.raises(ValueError):
         class_logprobs_grad(x, t, class_logprobs(x, t), torch.ones(4, device="cuda"), out=w)
+
+
+@pytest.mark.gpu
+def test_ids_that_64_bits_do_not_hold_are_refused():
+    """They do not come back as other classes."""
+    from trspmm import class_logprobs, class_logprobs_grad
+    x, t, one = _scores(4, 10, F32), torch.tensor([0, 3, 2, 0], device="cuda"), torch.ones(4, device="cuda")
+    r = class_logprobs(x, t)
+    for bad in (1 << 64, (1 << 64) + 3, 1 << 63, -(1 << 63), -(1 << 64) + 1):
+        for call in (lambda: class_logprobs(x, t, ignore_id=bad), lambda: class_logprobs_grad(x, t, r, one, ignore_id=bad)):
+            with pytest.raises(ValueError):
+                call()
+    for far in ((1 << 63) - 1, 1 - (1 << 63)):
+        assert torch.equal(class_logprobs(x, t, ignore_id=far).logprobs, r.logprobs)

@@ -43,6 +43,15 @@ def _check_ids(ids: torch.Tensor, index: int) -> int:
     return 1 if ids.dtype is torch.int64 else 0
 
 
+def _special_id(value, none: int, what: str) -> int:
+    """An id with a meaning of its own, as the C entry takes it (`none`, the lowest of 64 bits, where there is none)."""
+    if value is None:
+        return none
+    if not none < value < 1 << 63:   # ctypes would cut it to 64 bits: another id
+        raise ValueError(f"{what} must lie above -2^63 and below 2^63")
+    return value
+
+
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether the memory ranges of two strided matrices meet."""
     if a.numel() == 0 or b.numel() == 0:
@@ -99,7 +108,7 @@ def _lookup(table, ids, scale, padding_id, dtype, out):
             raise ValueError("out may not overlap the table or the ids")
         _written(out)
     _lib.launch(index, _lib.load().trs_embedding, table.data_ptr(), code, rows, stride, ids.data_ptr(), wide, ids.numel(), F, scale,
-                _NO_PADDING if padding_id is None else padding_id, out.data_ptr(), out_code, out_stride)
+                _special_id(padding_id, _NO_PADDING, "padding_id"), out.data_ptr(), out_code, out_stride)
     return out
 
 
@@ -183,5 +192,5 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: fl
     # the workspace is this call's own: calls on several streams, and graphs, do not share one
     ws = grad.new_empty(need.value, dtype=torch.uint8) if need.value else None
     _lib.launch(index, lib.trs_embedding_grad, grad.data_ptr(), code, stride, ids.data_ptr(), wide, n, n_rows, F, scale,
-                _NO_PADDING if padding_id is None else padding_id, out.data_ptr(), out_code, out_stride, 1 if accumulate else 0, None if ws is None else ws.data_ptr(), need.value)
+                _special_id(padding_id, _NO_PADDING, "padding_id"), out.data_ptr(), out_code, out_stride, 1 if accumulate else 0, None if ws is None else ws.data_ptr(), need.value)
     return out

@@ -12,7 +12,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .embedding import _check_out, _no_tangents, _overlap, _row_stride, _type_code, _written
+from .embedding import _check_out, _no_tangents, _overlap, _row_stride, _special_id, _type_code, _written
 
 MAX_TOP = 32
 _NO_IGNORE = -(1 << 63)
@@ -73,7 +73,7 @@ def _forward(logits, targets, top, mask, scale, ignore_id) -> ClassLogprobs:
     if top:
         top_logprobs = entropy.new_empty((n, top))
         top_ids = torch.empty_like(top_logprobs, dtype=torch.int32)
-    _lib.launch(index, _lib.load().trs_logprobs, *front, _NO_IGNORE if ignore_id is None else ignore_id, *back,
+    _lib.launch(index, _lib.load().trs_logprobs, *front, _special_id(ignore_id, _NO_IGNORE, "ignore_id"), *back,
                 None if logprobs is None else logprobs.data_ptr(), entropy.data_ptr(),
                 None if top_logprobs is None else top_logprobs.data_ptr(), None if top_ids is None else top_ids.data_ptr(),
                 stats.data_ptr())
@@ -81,7 +81,7 @@ def _forward(logits, targets, top, mask, scale, ignore_id) -> ClassLogprobs:
 
 
 def _launch_grad(index, front, back, ignore_id, top_ids, stats, entropy, g_logprobs, g_entropy, g_top, dx, dx_stride):
-    _lib.launch(index, _lib.load().trs_logprobs_grad, *front, _NO_IGNORE if ignore_id is None else ignore_id, *back,
+    _lib.launch(index, _lib.load().trs_logprobs_grad, *front, _special_id(ignore_id, _NO_IGNORE, "ignore_id"), *back,
                 None if g_top is None else top_ids.data_ptr(), stats.data_ptr(), None if g_entropy is None else entropy.data_ptr(),
                 None if g_logprobs is None else g_logprobs.data_ptr(), None if g_entropy is None else g_entropy.data_ptr(),
                 None if g_top is None else g_top.data_ptr(), dx.data_ptr(), dx_stride)
