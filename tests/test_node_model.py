@@ -145,3 +145,14 @@ def test_a_whole_step_captured_and_replayed():
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(held, step()))
+
+
+def test_classify_refuses_labels_of_another_graph():
+    """Labels are all nodes': a longer list is another graph's, and its first part not this one's."""
+    from trspmm import ShardedGCN2
+    rp, col, val, n, _ = _graph()
+    model = ShardedGCN2(rp, col, val)
+    X, W1, W2 = [torch.zeros(*s, dtype=torch.float16, device="cuda") for s in ((n, 16), (16, 16), (16, 8))]
+    for bad in (n + 1, n - 1, 2 * n):
+        with pytest.raises(ValueError):
+            model.classify(X, W1, W2, torch.zeros(bad, dtype=torch.int64, device="cuda"))

@@ -103,6 +103,8 @@ class ShardedGCN2:
                  gather: str = "h1", ids: torch.Tensor | None = None, ignore_id: int | None = None) -> ClassLogprobs:
         """The forward pass, and what its F2 outputs say as scores over F2 classes: for this rank's rows the log probabilities
         of their labels ([N], all nodes'), the entropies and the `top` best classes (class_logprobs)."""
+        if labels is not None and labels.shape != (self.n,):
+            raise ValueError(f"labels has shape {tuple(labels.shape)}, the graph {self.n} nodes")
         out = self.forward(X, W1, W2, gather, ids)
         own = None if labels is None else labels[self.r0:self.r1]
         return class_logprobs(out, own, top=top, ignore_id=ignore_id)
