@@ -383,7 +383,7 @@ int trs_embedding(const void* table, int table_type, long long rows, long long t
  * id names are left as they are.  Ids equal to padding_id and ids outside [0, rows) contribute nothing.  The positions are
  * sorted by id and summed in fp32 in an order that depends on the ids alone: no atomics, the same bits every time.
  * `workspace`: trs_embedding_grad_workspace_bytes of 16-byte aligned device memory that no overlapping call uses;
- * its contents need not be kept or cleared. */
+ * its contents need not be kept or cleared.  `out` may not overlap the gradient, the ids or the workspace. */
 int trs_embedding_grad_workspace_bytes(long long n, long long rows, int F, size_t* bytes);
 int trs_embedding_grad(const void* grad, int grad_type, long long grad_stride, const void* ids, int ids64, long long n,
                        long long rows, int F, float scale, long long padding_id, void* out, int out_type,
@@ -411,7 +411,8 @@ int trs_logprobs(const void* x, int type, long long n, int classes, long long st
  *   dx[r, j] = scale ( sum of g_c over the target and alternatives c = j  -  p_j (sum of all g_c + g_entropy (log p_j + entropy)) )
  * of x's type, 0 where masked, for rows in which no class is left and for rows whose weights are all 0; NaN (where not masked) in rows
  * in which the forward call gave NaN.  x and dx lie on element boundaries, in any alignment beyond that.
- * Ignored targets and those outside [0, classes) have no weight.  dx may not overlap x. */
+ * Ignored targets and those outside [0, classes) have no weight.  dx may not overlap x or any other array
+ * that the call reads. */
 int trs_logprobs_grad(const void* x, int type, long long n, int classes, long long stride, const void* targets, int targets64,
                       long long ignore_id, const unsigned char* mask, long long mask_stride, float scale, int top,
                       const int32_t* top_ids, const float* stats, const float* entropy, const float* g_logprobs,

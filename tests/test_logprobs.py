@@ -553,3 +553,27 @@ def test_ids_that_64_bits_do_not_hold_are_refused():
                 call()
     for far in ((1 << 63) - 1, 1 - (1 << 63)):
         assert torch.equal(class_logprobs(x, t, ignore_id=far).logprobs, r.logprobs)
+
+
+@pytest.mark.gpu
+def test_a_gradient_over_what_the_call_reads_is_refused():
+    """Rows are written while others still read their weights."""
+    from trspmm import class_logprobs, class_logprobs_grad
+    x, one = _scores(4, 10, F32), torch.ones(4, device="cuda")
+    t, mask = torch.tensor([0, 3, 2, 0], device="cuda"), torch.ones(4, 10, dtype=torch.bool, device="cuda")
+    r = class_logprobs(x, t, top=2, mask=mask)
+    two = torch.ones(4, 2, device="cuda")
+
+    def into(**what):   # all arguments apart from the one that lies in the result's memory
+        out = torch.zeros(4, 10, device="cuda")
+        a = dict(t=t, g=one, h=one, k=two, mask=mask, entropy=r.entropy, top_ids=r.top_ids, stats=r.stats)
+        for name in what:
+            v = a[name]
+            place = out.view(-1).view(v.dtype)[2:2 + v.numel()].view(v.shape)
+            a[name] = place.copy_(v)
+        return class_logprobs_grad(x, a["t"], r._replace(entropy=a["entropy"], top_ids=a["top_ids"], stats=a["stats"]), a["g"], a["h"], a["k"],
+                                   a["mask"], out=out)
+    assert torch.equal(into(), class_logprobs_grad(x, t, r, one, one, two, mask))
+    for name in ("t", "g", "h", "k", "mask", "entropy", "top_ids", "stats"):
+        with pytest.raises(ValueError):
+            into(**{name: True})

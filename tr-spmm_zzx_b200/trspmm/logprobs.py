@@ -162,8 +162,9 @@ def class_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor | None, resu
         out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     elif out.shape != logits.shape or out.dtype is not logits.dtype or out.get_device() != index:
         raise ValueError("out must have the logits' shape and type and be on their device")
-    elif _overlap(out, logits):
-        raise ValueError("out may not overlap the logits")
+    elif any(t is not None and _overlap(out, t) for t in (logits, targets, mask, g_logprobs, g_entropy, g_top_logprobs, result.entropy,
+                                                          result.top_ids, result.stats)):
+        raise ValueError("out may not overlap the logits or anything else that the call reads")
     else:
         dx_stride = _row_stride(out, "out")
         _written(out)
