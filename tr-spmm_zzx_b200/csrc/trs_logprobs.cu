@@ -923,7 +923,7 @@ __global__ void __launch_bounds__(kShortThreads) k_short_rows_grad(const Backwar
 // Lanes and pieces per lane that hold a row of so many pieces, and rows a group.  Longer ones are a CTA's: forward from 128 pieces on, the
 // gradient from 64 (2^27 fp16 scores, us: 1000 classes 136 by groups, 148 by CTAs; their gradient 194, 119; of 300 classes 379, 392).
 constexpr int kShortScores = 16, kShortPieces = 128, kShortPiecesGrad = 64;
-template <class T, class Fn>
+template <class T, int MOST, class Fn>   // MOST: pieces of the longest row
 int with_short(int pieces, long long n, Fn fn) {
     constexpr int PER = kShortScores / Row<T>::VEC;
     auto rows = [&](auto g, auto per) {
@@ -936,11 +936,13 @@ int with_short(int pieces, long long n, Fn fn) {
     if (pieces <= 2 * PER) return rows(std::integral_constant<int, 2>(), per);
     if (pieces <= 4 * PER) return rows(std::integral_constant<int, 4>(), per);
     if (pieces <= 8 * PER) return rows(std::integral_constant<int, 8>(), per);
-    if (pieces <= 16 * PER) return rows(std::integral_constant<int, 16>(), per);
-    if constexpr (32 * PER < kShortPieces) {
-        if (pieces > 32 * PER) return rows(std::integral_constant<int, 32>(), std::integral_constant<int, 2 * PER>());
+    if constexpr (MOST > 16 * PER) {
+        if constexpr (MOST > 32 * PER) {
+            if (pieces > 32 * PER) return rows(std::integral_constant<int, 32>(), std::integral_constant<int, 2 * PER>());
+        }
+        if (pieces > 16 * PER) return rows(std::integral_constant<int, 32>(), per);
     }
-    return rows(std::integral_constant<int, 32>(), per);
+    return rows(std::integral_constant<int, 16>(), per);
 }
 // Pieces of a row, wherever it begins.
 template <class T>
@@ -997,7 +999,7 @@ extern "C" int trs_logprobs(const void* x, int type, long long n, int classes, l
         using T = decltype(t);
         const int pieces = most_pieces<T>(classes);
         if (pieces <= kShortPieces)
-            return with_short<T>(pieces, n, [&](auto g, auto per, auto rows) {
+            return with_short<T, kShortPieces>(pieces, n, [&](auto g, auto per, auto rows) {
                 constexpr int G = decltype(g)::value, ROWS = decltype(rows)::value;
                 return launch(k_short_rows<T, G, decltype(per)::value, ROWS>, dim3((unsigned)ceil_div64(ceil_div64(n, ROWS) * G, kShortThreads)),
                               kShortThreads, 0, (cudaStream_t)stream, a);
@@ -1042,7 +1044,7 @@ extern "C" int trs_logprobs_grad(const void* x, int type, long long n, int class
         using T = decltype(t);
         const int pieces = most_pieces<T>(classes);
         if (pieces <= kShortPiecesGrad)
-            return with_short<T>(pieces, n, [&](auto g, auto per, auto rows) {
+            return with_short<T, kShortPiecesGrad>(pieces, n, [&](auto g, auto per, auto rows) {
                 constexpr int G = decltype(g)::value, ROWS = decltype(rows)::value;
                 return launch(k_short_rows_grad<T, G, decltype(per)::value, ROWS>,
                               dim3((unsigned)ceil_div64(ceil_div64(n, ROWS) * G, kShortThreads)), kShortThreads, 0, (cudaStream_t)stream, a);
