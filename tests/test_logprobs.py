@@ -577,3 +577,71 @@ def test_a_gradient_over_what_the_call_reads_is_refused():
     for name in ("t", "g", "h", "k", "mask", "entropy", "top_ids", "stats"):
         with pytest.raises(ValueError):
             into(**{name: True})
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("C", [3, 17, 20, 47, 100, 200, 300, 480, 900])
+@pytest.mark.parametrize("layout", ["plain", "apart", "masked"])
+def test_many_short_rows(C, dtype, layout):
+    """So many rows that a group of lanes does several of them one after the other, the last group fewer."""
+    from trspmm import class_logprobs, class_logprobs_grad
+    pieces = (C + 16 // dtype.itemsize - 1 + 16 // dtype.itemsize - 1) * dtype.itemsize // 16
+    n = (606_208 if pieces * 16 // dtype.itemsize <= 128 else 303_104 if pieces * 16 // dtype.itemsize <= 256 else 151_552) + 3
+    g = torch.Generator(device="cuda").manual_seed(C)
+    x = _scores(n, C, dtype, width=C + 3 if layout == "apart" else None, offset=1 if layout == "apart" else 0)
+    mask = None
+    if layout == "masked":
+        mask = torch.rand(n, C, generator=g, device="cuda") < 0.7
+        mask[5::11] = False
+    t = torch.randint(0, C, (n,), generator=g, device="cuda")
+    t[::7] = -1
+    top = min(C, 4)
+    w = [torch.randn(n, generator=g, device="cuda"), torch.randn(n, generator=g, device="cuda"), torch.randn(n, top, generator=g, device="cuda")]
+    r = class_logprobs(x, t, top=top, mask=mask, scale=0.75, ignore_id=-1)
+    d = class_logprobs_grad(x, t, r, *w, mask=mask, scale=0.75, ignore_id=-1)
+    pick = torch.cat([torch.arange(2000), torch.arange(n - 2000, n), torch.randint(0, n, (2000,))]).cuda()
+    part = type(r)(*[v[pick] for v in r])
+    Ref(x[pick], t[pick], top, None if mask is None else mask[pick], 0.75, -1).check(part, d[pick], [v[pick] for v in w])
+    # the other rows: the same bits as by calls of few rows, in which a group has one
+    for a in range(0, n, 100_000):
+        b = min(a + 100_000, n)
+        m = None if mask is None else mask[a:b]
+        few = class_logprobs(x[a:b], t[a:b], top=top, mask=m, scale=0.75, ignore_id=-1)
+        assert all(torch.equal(p.view(torch.int32), q[a:b].view(torch.int32)) for p, q in zip(few, r))
+        again = class_logprobs_grad(x[a:b], t[a:b], few, *[v[a:b] for v in w], mask=m, scale=0.75, ignore_id=-1)
+        assert torch.equal(again.view(torch.int16), d[a:b].view(torch.int16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("n,C", [(4739, 1100), (4739, 2000), (2371, 6000), (1187, 30_000), (600, 70_001)])
+def test_many_long_rows(n, C, dtype):
+    """So many rows that each has few threads, down to one warp; values that crowd the alternatives' lists."""
+    from trspmm import class_logprobs, class_logprobs_grad
+    i = torch.arange(C, device="cuda")
+    vec = 16 // dtype.itemsize
+    g = torch.Generator(device="cuda").manual_seed(C)
+    for kind in ("random", "equal", "few values", "one lane", "one lane, equal", "masked", "apart"):
+        x = _scores(n, C, dtype, width=C + 5 if kind == "apart" else None, offset=3 if kind == "apart" else 0)
+        mask = None
+        lane = i // vec % 32 == 5   # places that one thread of a warp has
+        if kind == "equal":
+            x.fill_(2.5)
+        elif kind == "few values":
+            x.copy_(((i * 7919) % 5).to(dtype))
+        elif kind == "one lane":
+            x[:, lane] += 20
+        elif kind == "one lane, equal":
+            x[:, lane] = 20
+        elif kind == "masked":
+            mask = torch.rand(n, C, generator=g, device="cuda") < 0.7
+            mask[3::5] = False
+        t = torch.randint(0, C, (n,), generator=g, device="cuda")
+        t[::7] = -1
+        w = [torch.randn(n, generator=g, device="cuda"), torch.randn(n, generator=g, device="cuda"), torch.randn(n, 9, generator=g, device="cuda")]
+        r = class_logprobs(x, t, top=9, mask=mask, ignore_id=-1)
+        d = class_logprobs_grad(x, t, r, *w, mask=mask, ignore_id=-1)
+        for pick in (torch.arange(100, device="cuda"), torch.arange(n - 100, n, device="cuda")):
+            part = type(r)(*[v[pick] for v in r])
+            Ref(x[pick], t[pick], 9, None if mask is None else mask[pick], 1.0, -1).check(part, d[pick], [v[pick] for v in w])

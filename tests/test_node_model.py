@@ -156,3 +156,18 @@ def test_classify_refuses_labels_of_another_graph():
     for bad in (n + 1, n - 1, 2 * n):
         with pytest.raises(ValueError):
             model.classify(X, W1, W2, torch.zeros(bad, dtype=torch.int64, device="cuda"))
+
+
+def test_create_graph_gives_the_same_first_order_gradients():
+    """Every upstream gradient arrives, in its place, through the form that runs under create_graph."""
+    from trspmm import class_logprobs, embedding
+    g = torch.Generator(device="cuda").manual_seed(0)
+    W = torch.randn(40, 24, generator=g, device="cuda", requires_grad=True)
+    ids = torch.randint(0, 40, (90,), generator=g, device="cuda")
+    a, b, c = [torch.randn(*s, generator=g, device="cuda") for s in ((90,), (90,), (90, 3))]
+
+    def grad(create_graph):
+        r = class_logprobs(embedding(W, ids, scale=0.5, padding_id=3), ids % 24, top=3, scale=1.5, ignore_id=5)
+        loss = (r.logprobs * a).sum() + (r.entropy * b).sum() + (r.top_logprobs * c).sum()
+        return torch.autograd.grad(loss, W, create_graph=create_graph)[0]
+    assert torch.equal(grad(True).detach(), grad(False))
