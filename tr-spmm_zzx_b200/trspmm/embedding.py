@@ -43,11 +43,9 @@ def _check_ids(ids: torch.Tensor, index: int) -> int:
     return 1 if ids.dtype is torch.int64 else 0
 
 
-def _special_id(value, none: int, what: str) -> int:
-    """An id with a meaning of its own, as the C entry takes it (`none`, the lowest of 64 bits, where there is none)."""
-    if value is None:
-        return none
-    if not none < value < 1 << 63:   # ctypes would cut it to 64 bits: another id
+def _special_id(value, what: str) -> int:
+    """An id with a meaning of its own (the lowest of 64 bits tells the C entry that there is none)."""
+    if not -(1 << 63) < value < 1 << 63:   # ctypes would cut it to 64 bits: another id
         raise ValueError(f"{what} must lie above -2^63 and below 2^63")
     return value
 
@@ -64,9 +62,9 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 def _no_tangents(what: str, *tensors) -> None:
-    """Refuses tensors with a tangent: there is no forward-mode derivative, and the kernels would drop it in silence.  (Outside a
-    level of forward_ad, where there are none, this is one comparison.)"""
-    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+    """Refuses tensors with a tangent: there is no forward-mode derivative, and the kernels would drop it in silence.  (Callers ask
+    for the level first: outside one there are no tangents, and small calls notice every function.)"""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
@@ -76,7 +74,7 @@ def _written(out: torch.Tensor) -> None:
 
 
 def _check_out(what: str, out) -> None:
-    if out is not None and out.requires_grad and torch.is_grad_enabled():
+    if out.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what} with out= is not differentiable: call it under torch.no_grad()")
 
 
@@ -108,7 +106,7 @@ def _lookup(table, ids, scale, padding_id, dtype, out):
             raise ValueError("out may not overlap the table or the ids")
         _written(out)
     _lib.launch(index, _lib.load().trs_embedding, table.data_ptr(), code, rows, stride, ids.data_ptr(), wide, ids.numel(), F, scale,
-                _special_id(padding_id, _NO_PADDING, "padding_id"), out.data_ptr(), out_code, out_stride)
+                _NO_PADDING if padding_id is None else _special_id(padding_id, "padding_id"), out.data_ptr(), out_code, out_stride)
     return out
 
 
@@ -138,8 +136,10 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, paddin
     the fp16 features that the SpMM takes without a copy of the table.  `out` may be given instead (for a vector of ids its rows
     may lie apart).  Differentiable in the table where no `out` is given: the gradient is embedding_grad's, dense, in the
     table's type.  Forward-mode differentiation is refused."""
-    _no_tangents("embedding", table, out)
-    _check_out("embedding", out)
+    if forward_ad._current_level >= 0:
+        _no_tangents("embedding", table, out)
+    if out is not None:
+        _check_out("embedding", out)
     if table.requires_grad and torch.is_grad_enabled():
         if out is not None:
             raise ValueError("embedding with out= is not differentiable: call it under torch.no_grad()")
@@ -157,8 +157,10 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: fl
     once to out_dtype (the type of `grad` unless given).  Rows that no id names are zero.  With `accumulate` the sums
     are added to `out`, whose other rows stay as they are (micro-batches).  Padding ids and ids outside the table contribute
     nothing."""
-    _no_tangents("embedding_grad", grad, out)
-    _check_out("embedding_grad", out)
+    if forward_ad._current_level >= 0:
+        _no_tangents("embedding_grad", grad, out)
+    if out is not None:
+        _check_out("embedding_grad", out)
     index = grad.get_device()
     if index < 0:
         raise ValueError("embedding_grad needs CUDA tensors (there is no CPU fallback)")
@@ -192,5 +194,5 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: fl
     # the workspace is this call's own: calls on several streams, and graphs, do not share one
     ws = grad.new_empty(need.value, dtype=torch.uint8) if need.value else None
     _lib.launch(index, lib.trs_embedding_grad, grad.data_ptr(), code, stride, ids.data_ptr(), wide, n, n_rows, F, scale,
-                _special_id(padding_id, _NO_PADDING, "padding_id"), out.data_ptr(), out_code, out_stride, 1 if accumulate else 0, None if ws is None else ws.data_ptr(), need.value)
+                _NO_PADDING if padding_id is None else _special_id(padding_id, "padding_id"), out.data_ptr(), out_code, out_stride, 1 if accumulate else 0, None if ws is None else ws.data_ptr(), need.value)
     return out

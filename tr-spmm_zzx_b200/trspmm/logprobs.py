@@ -10,6 +10,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .embedding import _check_out, _no_tangents, _overlap, _row_stride, _special_id, _type_code, _written
@@ -73,7 +74,7 @@ def _forward(logits, targets, top, mask, scale, ignore_id) -> ClassLogprobs:
     if top:
         top_logprobs = entropy.new_empty((n, top))
         top_ids = torch.empty_like(top_logprobs, dtype=torch.int32)
-    _lib.launch(index, _lib.load().trs_logprobs, *front, _special_id(ignore_id, _NO_IGNORE, "ignore_id"), *back,
+    _lib.launch(index, _lib.load().trs_logprobs, *front, _NO_IGNORE if ignore_id is None else _special_id(ignore_id, "ignore_id"), *back,
                 None if logprobs is None else logprobs.data_ptr(), entropy.data_ptr(),
                 None if top_logprobs is None else top_logprobs.data_ptr(), None if top_ids is None else top_ids.data_ptr(),
                 stats.data_ptr())
@@ -81,7 +82,7 @@ def _forward(logits, targets, top, mask, scale, ignore_id) -> ClassLogprobs:
 
 
 def _launch_grad(index, front, back, ignore_id, top_ids, stats, entropy, g_logprobs, g_entropy, g_top, dx, dx_stride):
-    _lib.launch(index, _lib.load().trs_logprobs_grad, *front, _special_id(ignore_id, _NO_IGNORE, "ignore_id"), *back,
+    _lib.launch(index, _lib.load().trs_logprobs_grad, *front, _NO_IGNORE if ignore_id is None else _special_id(ignore_id, "ignore_id"), *back,
                 None if g_top is None else top_ids.data_ptr(), stats.data_ptr(), None if g_entropy is None else entropy.data_ptr(),
                 None if g_logprobs is None else g_logprobs.data_ptr(), None if g_entropy is None else g_entropy.data_ptr(),
                 None if g_top is None else g_top.data_ptr(), dx.data_ptr(), dx_stride)
@@ -101,7 +102,8 @@ class _LogprobsFn(torch.autograd.Function):
     def backward(ctx, g_logprobs, g_entropy, g_top, _ids, _stats):
         if torch.is_grad_enabled():   # under create_graph
             return _LogprobsFn.once(ctx, g_logprobs, g_entropy, g_top, _ids, _stats)
-        _no_tangents("the gradient of class_logprobs", g_logprobs, g_entropy, g_top)
+        if forward_ad._current_level >= 0:
+            _no_tangents("the gradient of class_logprobs", g_logprobs, g_entropy, g_top)
         logits, targets, mask, entropy, top_ids, stats = ctx.saved_tensors
         scale, ignore_id = ctx.args
         if g_logprobs is None and g_entropy is None and g_top is None:
@@ -128,7 +130,8 @@ def class_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
 
     Differentiable in the logits through logprobs, entropy and top_logprobs (not through the choice of the alternatives).  Forward-mode
     differentiation is refused."""
-    _no_tangents("class_logprobs", logits)
+    if forward_ad._current_level >= 0:
+        _no_tangents("class_logprobs", logits)
     if logits.requires_grad and torch.is_grad_enabled():
         return ClassLogprobs(*_LogprobsFn.apply(logits, targets, top, mask, scale, ignore_id))
     return _forward(logits, targets, top, mask, scale, ignore_id)
@@ -141,8 +144,10 @@ def class_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor | None, resu
     """The gradient of the logits, of their shape and type, from the gradients (fp32, contiguous) of what class_logprobs
     returned for the same arguments as `result` (its entropy is read where g_entropy is given, its top_ids where g_top_logprobs
     is, its stats always)."""
-    _no_tangents("class_logprobs_grad", logits, result.stats, result.entropy, g_logprobs, g_entropy, g_top_logprobs, out)
-    _check_out("class_logprobs_grad", out)
+    if forward_ad._current_level >= 0:
+        _no_tangents("class_logprobs_grad", logits, result.stats, result.entropy, g_logprobs, g_entropy, g_top_logprobs, out)
+    if out is not None:
+        _check_out("class_logprobs_grad", out)
     top = 0 if g_top_logprobs is None else g_top_logprobs.shape[-1]
     index, front, back = _check(logits, targets, mask, scale, top)
     n = logits.shape[0]
