@@ -401,7 +401,8 @@ int trs_embedding_grad(const void* grad, int grad_type, long long grad_stride, c
  * in which no class is left gives -inf, entropy 0 and alternatives -1 with -inf (as do alternatives beyond the number of
  * classes left); a row in which a NaN or +inf is left gives NaN and alternatives -1.  Each output may be NULL
  * (top_ids and top_logprobs only when top = 0, stats: 8-byte aligned).  scale > 0 and below 2e38, top <= 32, classes <= 2^30,
- * n < 2^31.  fp32 arithmetic whatever the type.  Asynchronous on `stream`; no workspace, allocates nothing. */
+ * n < 2^31.  fp32 arithmetic whatever the type: a score further than 3.4e38 below the row's
+ * largest counts as infinitely far.  Asynchronous on `stream`; no workspace, allocates nothing. */
 #define TRS_NO_IGNORE INT64_MIN
 int trs_logprobs(const void* x, int type, long long n, int classes, long long stride, const void* targets, int targets64,
                  long long ignore_id, const unsigned char* mask, long long mask_stride, float scale, int top,
@@ -409,7 +410,7 @@ int trs_logprobs(const void* x, int type, long long n, int classes, long long st
 /* Gradient of the scores: from g_* = gradients of logprobs [n], entropy [n] and top_logprobs [n, top] (each may be NULL: 0),
  * and the forward call's inputs and outputs (entropy is read where g_entropy is given, top_ids where g_top_logprobs is):
  *   dx[r, j] = scale ( sum of g_c over the target and alternatives c = j  -  p_j (sum of all g_c + g_entropy (log p_j + entropy)) )
- * of x's type, 0 where masked, for rows in which no class is left and for rows whose weights are all 0; NaN (where not masked) in rows
+ * of x's type, 0 where masked, for rows in which no class is left and for rows in which every weight is 0; NaN (where not masked) in rows
  * in which the forward call gave NaN.  x and dx lie on element boundaries, in any alignment beyond that.
  * Ignored targets and those outside [0, classes) have no weight.  dx may not overlap x or any other array
  * that the call reads. */

@@ -72,8 +72,8 @@ __global__ void __launch_bounds__(kLookupThreads, 8) k_lookup(const TI* __restri
 // Positions sorted by id
 // ----------------------------------------------------------------------------------------------
 // Stable, so that a row's positions ascend.  Positions without a row (padding, outside the table) get the key `rows` and come last.
-// The keys have bits(rows) bits, sorted by up to 11 (many ids: 8) at a time: two passes for tables of up to 4 M rows.  Pass: the counts of
-// each digit in each tile, their prefix sums over the tiles, then every key to its place.
+// The keys have bits(rows) bits, sorted by up to 11 (from 2^19 ids on: 8) at a time: two (three) passes for tables of up to 4 M rows.
+// Pass: the counts of each digit in each tile, their prefix sums over the tiles, then every key to its place.
 constexpr int kSortThreads = 512, kSortWarps = kSortThreads / 32, kSortItems = 8, kTile = kSortThreads * kSortItems, kMaxDigit = 11;
 
 __device__ __forceinline__ unsigned key_of(long long id, long long rows, long long padding) {
@@ -326,9 +326,9 @@ __global__ void __launch_bounds__(kSortThreads) k_sort_few(const void* __restric
 // The sorted positions are cut into blocks of 64 and spans of several blocks.  A block whose positions all name one row is summed
 // ahead (a span of one row as a whole), all of them in parallel, so that a row with a hundred thousand positions is not one
 // group's work.  Rows with kPopular positions or more are noted in a list (popular[0] of them, in any order) and get a CTA each, the
-// first ones of k_sums: as part of their neighbours' work a hub was its last 60 us where others were done, and a table whose rows are in
-// the order of their popularity took 336 us where the same ids spread over it took 196 (now 197; from 16 positions on 184, but 600 k ids of
-// 50 k rows 99 us for 74).
+// first ones of k_sums: as part of their neighbours' work a hub was its last 60 us where others were done, and 2^20 popular ids of a table
+// whose rows are in the order of their popularity took 336 us where the same ids spread over it took 196 (now 197 and 195; from 16 positions
+// on 184, but 600 k ids of 50 k rows 99 us for 77).
 constexpr int kBlock = 64, kSpanWarps = kThreads / 32, kPopular = 24;
 
 template <class T, int VEC>
@@ -362,7 +362,9 @@ __device__ __forceinline__ void sum_block(float (&acc)[VEC], const T* __restrict
         for (int k = 0; k < VEC; ++k) acc[k] += __shfl_xor_sync(0xffffffffu, acc[k], o);
 }
 
-// One CTA a span: notes where segments begin and end, and sums its uniform blocks.
+// One CTA a span: notes where segments begin and end, and sums its uniform blocks.  (Four CTAs an SM leave 64 registers, and what the
+// compiler wants beyond them lies in local memory: 64 to 80 bytes a thread for fp16 in pieces of eight, about 250 for bf16, 728 for single
+// fp32 elements by 32 lanes.  The bound was chosen on fp16; the whole gradient of 2^20 bf16 rows of 128 takes 195 us as that of fp16 does.)
 template <class T, int VEC, int G>
 __global__ void __launch_bounds__(kThreads, 4) k_block_sums(const T* __restrict__ g, long long stride, const uint2* __restrict__ words, int n, unsigned rows, int F, int span,
                                                          int2* __restrict__ segment, float* __restrict__ block_sum,
@@ -605,8 +607,9 @@ int with_group(int pieces, Fn fn) {
 }
 
 // Lookup: lanes, rows and pieces in flight.  Few lanes a row spare instructions (what a lane spends on a row's id and address is as much
-// as it spends on three pieces): F = 47 of fp32 rows 27 us with 32 lanes x 4 rows, 17 us with 16 lanes x 2 rows x 3 pieces.  The kernel keeps to
-// 64 registers: 2^20 rows of 128 fp16 features 77 us with 66 of them, 66 with 64, 79 with 40.
+// as it spends on three pieces): F = 47 of fp32 rows, single elements as in all odd widths, 27 us with 32 lanes x 4 rows, 17 us with
+// 16 lanes x 2 rows x 3 pieces.  That fits 33 to 48 pieces; longer rows take further turns of 48, in the last of which lanes without a piece load the
+// row's last one again.  The kernel keeps to 64 registers: 2^20 rows of 128 fp16 features 77 us with 66 of them, 66 with 64, 79 with 40.
 template <class Fn>
 int with_lookup(int pieces, Fn fn) {
     using std::integral_constant;

@@ -4,7 +4,8 @@
 // T = sum e^(d_j) d_j:
 //   log p_j = d_j - log S,   entropy = log S - T / S,   alternatives: the largest x_j, the lowest class first among equal ones.
 // A row is read once; m, S and T are carried along it and rescaled when m grows.  Differences to m are taken before the scale, so
-// rows of the type's lowest value stay exact.  Everything is held in fp32.
+// rows of the type's lowest value stay exact; a score whose distance to m leaves fp32's range (3.4e38) counts as infinitely far.  Everything is
+// held in fp32.
 //   no class left:        log probability -inf, entropy 0, alternatives -1 with -inf, gradient 0
 //   NaN or +inf left:     NaN (alternatives -1), gradient NaN
 //   target = ignore id:   log probability 0, no gradient of it;   target outside [0, classes): NaN, no gradient of it
@@ -42,6 +43,9 @@ __device__ __forceinline__ float key_score(Key k) {
 }
 __device__ __forceinline__ int key_class(Key k) { return (int)~(unsigned)k; }
 
+// e^(d) as 2^(d log2 e) by the special-function unit: two instructions a score, where the library's function takes several and the
+// forward pass is bound by them.  The argument is rounded once after its factor, so a class |z| below the best has a probability off by up to
+// |z| 2^-24 of itself beside the unit's 2^-22; what is that far down hardly counts in the sums.
 __device__ __forceinline__ float exp_2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -821,7 +825,9 @@ __global__ void __launch_bounds__(THREADS) k_row_grad(const Backward a, int part
     T* dx = (T*)a.dx + r * a.dx_stride;
     const RowGrad g = row_grad(a, r);
     const int per = (row.pieces + parts - 1) / parts, p0 = min(row.pieces, part * per), p1 = min(row.pieces, p0 + per);
-    // whole pieces whose places in dx are aligned as in x
+    // Whole pieces whose places in dx are aligned as in x.  Where they are not (scores cut from a padded product, and a dx without gaps) the
+    // row goes by write_piece, its stores element by element: 4096 rows of 50021 bf16 scores, 50024 apart, 533 us; into a dx with the same
+    // gaps 134, as without gaps on both sides.
     const bool straight = (uintptr_t)(dx - row.head) % 16 == 0;
     const bool broken = MASKED && g.inv_S != g.inv_S;   // what is masked is 0 even there: piece by piece
     const int q0 = straight && !broken ? max(p0, row.head ? 1 : 0) : p1, q1 = min(p1, (row.head + row.classes) / VEC);
@@ -1011,7 +1017,7 @@ extern "C" int trs_logprobs(const void* x, int type, long long n, int classes, l
         };
         // As few threads a row as keep it going, many rows at a time: what a row costs beside its scores grows with its threads.  2^27 fp16
         // scores by 32 / 64 / 128 / 256 threads, us: 2000 classes 99 / 122 / 146 / 247, 9000: 67 / 56 / 62 / 87, 33000:
-        // 70 / 54 / 52 / 56; fp32 33000: 89 / 99 / 93 / 97.
+        // 70 / 54 / 52 / 56; 2^27 fp32 scores in rows of 33000: 89 / 99 / 93 / 97.
         int threads = sizeof(T) == 4 ? (pieces <= 8192 ? 32 : 256) : pieces <= 640 ? 32 : pieces <= 2400 ? 64 : pieces <= 8192 ? 128 : 256;
         while (threads < 256 && n * threads < 148 * 1024 && pieces > threads * kTurn) threads *= 2;   // unless rows are few
         if (threads == 32) return run(std::integral_constant<int, 32>(), 1);
